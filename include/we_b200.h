@@ -76,7 +76,9 @@ enum {
 enum {
   WE_B200_ST_OK = 0,
   WE_B200_ST_WAIT_EXPIRED = 1, /* a bounded mbarrier wait gave up; output invalid */
-  WE_B200_ST_INDEX_RANGE = 2   /* a token position points outside the RoPE table (the row was clamped) */
+  WE_B200_ST_INDEX_RANGE = 2,  /* a token position points outside the RoPE table (the row was clamped) */
+  WE_B200_ST_PAGE_RANGE = 3    /* a page index or a token count of a paged cache is out of range (the token was
+                                  dropped, or page 0 read in its place) */
 };
 
 typedef struct we_b200_cache_geom {
@@ -258,6 +260,116 @@ typedef struct we_b200_prologue_args {
 } we_b200_prologue_args;
 
 WE_B200_API int we_b200_qkv_prologue(const we_b200_prologue_args* args_host, int32_t* status, void* stream);
+
+/* ------------------------------------------------------------------ paged cache
+ * Sessions that grow token by token, at lengths of their own: the K/V rows of a
+ * layer lie in a pool of pages, kv[2, P, Hkv, page, Dh], and row s of `table`
+ * lists the pages of session s in the order of its tokens (token i of kv head h:
+ * page table[s][i / page], row i % page).  (No counterpart in the reference,
+ * whose cache overwrites the oldest frame of a ring, src/model/kv_cache.py:64-154.)
+ *
+ * `lens[S][Hkv]` counts the tokens a kv head holds and `next_pos[S][Hkv]` the
+ * tokens it was ever given (= the position of the next one).  With eviction the
+ * tokens a head holds are its own choice: `weights[P][Hkv][page]` is the softmax
+ * weight a token has been given so far (summed over the query heads that share
+ * the kv head, added up by we_b200_paged_attn) and `positions[P][Hkv][page]`
+ * the position it came with.  All of them int32 / float32, contiguous.
+ *
+ * A page belongs to one session where anything is written (append, eviction);
+ * sessions may share pages they only read, and the weights of shared pages add
+ * up (in an order that is not fixed).  Page indexes outside [0, P), counts
+ * below 0 and tokens beyond max_pages * page set *status to
+ * WE_B200_ST_PAGE_RANGE; nothing out of range is read or written.
+ */
+typedef struct we_b200_paged_geom {
+  int32_t S;                    /* sessions                                         */
+  int32_t Hkv;                  /* kv heads                                         */
+  int32_t Dh;                   /* head dim: 64 or 128                              */
+  int32_t page;                 /* tokens per page: 16, 32, 64, 128 or 256          */
+  int32_t n_pages;              /* P, pages of the pool                             */
+  int32_t max_pages;            /* table entries per session                        */
+  int32_t dtype;                /* WE_B200_BF16 or WE_B200_F16                      */
+  int32_t reserved;
+  int64_t plane_stride;         /* elements of kv between the K and the V plane     */
+  int64_t page_stride;          /* ... between pages                                */
+  int64_t head_stride;          /* ... between kv heads                             */
+  int64_t token_stride;         /* ... between the rows of a page                   */
+  int64_t table_stride;         /* int32 entries between the sessions' table rows   */
+} we_b200_paged_geom;
+
+typedef struct we_b200_paged_append_args {
+  we_b200_paged_geom geom;
+  const void* k_new;            /* [S, Hkv, T, Dh] views, strides (s, h, t); may be */
+  const void* v_new;            /* NULL when T is 0                                 */
+  int64_t k_strides[3], v_strides[3];
+  void* kv;
+  float* weights;               /* may be NULL (append without eviction)            */
+  int32_t* positions;           /* may be NULL (append without eviction)            */
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* next_pos;
+  int32_t* lens_out;            /* may be `lens` itself                             */
+  int32_t* next_pos_out;        /* may be `next_pos` itself                         */
+  const int32_t* n_new;         /* [S]: tokens of each session among the T, or NULL: all T */
+  const float* w_new;           /* [S, Hkv, T] view: weights the new tokens come with, or NULL: 0 */
+  int64_t w_strides[3];
+  void* workspace;              /* we_b200_paged_append_evict only                  */
+  uint64_t workspace_bytes;
+  int32_t T;
+  int32_t keep, sink, recent;   /* we_b200_paged_append_evict only                  */
+} we_b200_paged_append_args;
+
+/*
+ * Appends n_new[s] tokens to every kv head of session s: token t goes to slot
+ * lens[s][h] + t, its weight becomes w_new or 0, its position next_pos[s][h] + t.
+ * lens_out / next_pos_out receive the counts after it.  Rows t >= n_new[s] of
+ * the new tokens are not read (a padded batch).
+ */
+WE_B200_API int we_b200_paged_append(const we_b200_paged_append_args* args_host, int32_t* status, void* stream);
+
+/*
+ * The same under a budget: afterwards no kv head holds more than `keep` tokens.
+ * Candidates are the held tokens (index 0 .. len) and then the new ones
+ * (len .. len + n).  Shielded are positions < sink and the last `recent`
+ * positions (sink + recent <= keep).  Kept are the `keep` best by: shielded
+ * first, then the larger weight (NaN counts as the largest), then the lower
+ * index.  Kept tokens of an index >= keep move to the indexes < keep that the
+ * evicted ones left, both in ascending order; the others stay where they are,
+ * so little is moved.  What an evicted slot beyond the budget holds is left as
+ * it was.  The workspace (we_b200_paged_evict_workspace_bytes) needs no
+ * initialisation.
+ */
+WE_B200_API int we_b200_paged_append_evict(const we_b200_paged_append_args* args_host, int32_t* status, void* stream);
+WE_B200_API size_t we_b200_paged_evict_workspace_bytes(const we_b200_paged_geom* geom_host, int32_t T, int32_t keep);
+
+typedef struct we_b200_paged_attn_args {
+  we_b200_paged_geom geom;
+  const void* q;                /* [S, Hq, Dh] view, strides (s, h)                 */
+  void* out;                    /* [S, Hq, Dh] view, strides (s, h)                 */
+  int64_t q_strides[2], out_strides[2];
+  const void* kv;
+  const int32_t* table;
+  const int32_t* lens;
+  float* weights;               /* NULL: the weights are not added up               */
+  float* lse;                   /* [S][Hq] fp32, contiguous, or NULL                */
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t Hq;
+  float scale;                  /* <= 0: 1/sqrt(Dh)                                 */
+} we_b200_paged_attn_args;
+
+/*
+ * Attention of one new token per session over its paged cache:
+ *   out[s,g] = sum_j p_gj v_j,  p_g = softmax(scale * q_g . k_j) over j < lens[s][h]
+ * for every query head g of kv head h = g / (Hq / Hkv).  With `weights`, the
+ * token j of kv head h has sum_g p_gj added to its weight; with `lse`, the
+ * logarithm of the softmax sum (natural units) is stored.  A head that holds
+ * nothing gives 0 and -inf.  Workspace: we_b200_paged_attn_workspace_bytes,
+ * contents irrelevant before and after.
+ */
+WE_B200_API int we_b200_paged_attn(const we_b200_paged_attn_args* args_host, int32_t* status, void* stream);
+WE_B200_API size_t we_b200_paged_attn_workspace_bytes(const we_b200_paged_geom* geom_host, int32_t Hq,
+                                                      int accumulate);
 
 /* Number of kernels the previous three entry points have launched in this
  * process (diagnostic counter for benchmarks; relaxed atomics). */

@@ -27,6 +27,11 @@ EXPORTS = (
     "we_b200_append_attend_gated",
     "we_b200_frame_attn_static",
     "we_b200_qkv_prologue",
+    "we_b200_paged_append",
+    "we_b200_paged_append_evict",
+    "we_b200_paged_evict_workspace_bytes",
+    "we_b200_paged_attn",
+    "we_b200_paged_attn_workspace_bytes",
     "we_b200_launch_count",
 )
 
@@ -57,6 +62,44 @@ class PrologueArgs(ctypes.Structure):
         ("height", c_int32), ("width", c_int32),
         ("B", c_int32), ("T", c_int32), ("Hq", c_int32), ("Hkv", c_int32), ("Dh", c_int32),
         ("dtype", c_int32), ("eps", c_float),
+    ]
+
+
+Strides2 = c_int64 * 2
+
+
+class PagedGeom(ctypes.Structure):
+    """Mirror of `we_b200_paged_geom`."""
+    _fields_ = [
+        ("S", c_int32), ("Hkv", c_int32), ("Dh", c_int32), ("page", c_int32),
+        ("n_pages", c_int32), ("max_pages", c_int32), ("dtype", c_int32), ("reserved", c_int32),
+        ("plane_stride", c_int64), ("page_stride", c_int64), ("head_stride", c_int64), ("token_stride", c_int64),
+        ("table_stride", c_int64),
+    ]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    """Mirror of `we_b200_paged_append_args`."""
+    _fields_ = [
+        ("geom", PagedGeom),
+        ("k_new", c_void_p), ("v_new", c_void_p), ("k_strides", Strides3), ("v_strides", Strides3),
+        ("kv", c_void_p), ("weights", c_void_p), ("positions", c_void_p),
+        ("table", c_void_p), ("lens", c_void_p), ("next_pos", c_void_p),
+        ("lens_out", c_void_p), ("next_pos_out", c_void_p),
+        ("n_new", c_void_p), ("w_new", c_void_p), ("w_strides", Strides3),
+        ("workspace", c_void_p), ("workspace_bytes", c_uint64),
+        ("T", c_int32), ("keep", c_int32), ("sink", c_int32), ("recent", c_int32),
+    ]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    """Mirror of `we_b200_paged_attn_args`."""
+    _fields_ = [
+        ("geom", PagedGeom),
+        ("q", c_void_p), ("out", c_void_p), ("q_strides", Strides2), ("out_strides", Strides2),
+        ("kv", c_void_p), ("table", c_void_p), ("lens", c_void_p), ("weights", c_void_p), ("lse", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_uint64),
+        ("Hq", c_int32), ("scale", c_float),
     ]
 
 
@@ -130,6 +173,17 @@ def load() -> ctypes.CDLL:
 
     lib.we_b200_qkv_prologue.restype = c_int
     lib.we_b200_qkv_prologue.argtypes = [POINTER(PrologueArgs), c_void_p, c_void_p]
+
+    for name in ("we_b200_paged_append", "we_b200_paged_append_evict"):
+        fn = getattr(lib, name)
+        fn.restype = c_int
+        fn.argtypes = [POINTER(PagedAppendArgs), c_void_p, c_void_p]
+    lib.we_b200_paged_evict_workspace_bytes.restype = c_size_t
+    lib.we_b200_paged_evict_workspace_bytes.argtypes = [POINTER(PagedGeom), c_int32, c_int32]
+    lib.we_b200_paged_attn.restype = c_int
+    lib.we_b200_paged_attn.argtypes = [POINTER(PagedAttnArgs), c_void_p, c_void_p]
+    lib.we_b200_paged_attn_workspace_bytes.restype = c_size_t
+    lib.we_b200_paged_attn_workspace_bytes.argtypes = [POINTER(PagedGeom), c_int32, c_int]
 
     got = lib.we_b200_abi_version()
     if got != ABI_VERSION:

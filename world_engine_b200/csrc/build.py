@@ -11,8 +11,9 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
-SOURCES = ["abi.cu", "kv_append.cu", "block_mask.cu", "frame_attn.cu", "qkv_prologue.cu"]
-HEADERS = ["common.cuh", "ptx.cuh", os.path.join("..", "..", "include", "we_b200.h")]
+SOURCES = ["abi.cu", "kv_append.cu", "block_mask.cu", "frame_attn.cu", "qkv_prologue.cu", "paged_append.cu",
+           "paged_attn.cu"]
+HEADERS = ["common.cuh", "ptx.cuh", "paged.cuh", os.path.join("..", "..", "include", "we_b200.h")]
 
 
 def lib_path(debug: bool = False) -> str:

@@ -9,12 +9,13 @@ split-KV workspace and the status word.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import CacheGeom, PrologueArgs, Strides3
+from ._lib import CacheGeom, PagedAppendArgs, PagedAttnArgs, PagedGeom, PrologueArgs, Strides3
 
 _DTYPE_CODE = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
 
@@ -95,7 +96,8 @@ def check_status(device: torch.device) -> None:
     if st != 0:
         status_word(device).zero_()
         what = {1: "a bounded wait of the attention kernel expired; the output of that call is invalid",
-                2: "a token position points outside the RoPE table (IndexError in the reference)"}.get(st & 0xFF, "unknown")
+                2: "a token position points outside the RoPE table (IndexError in the reference)",
+                3: "a page index or a token count of a paged cache is out of range"}.get(st & 0xFF, "unknown")
         where = f" (debug build: wait at source line {st >> 8})" if st >> 8 else ""
         raise RuntimeError(f"world_engine_b200: device status {st & 0xFF}: {what}{where}")
 
@@ -259,6 +261,140 @@ def block_mask_tables(mask_written: torch.Tensor, tokens_per_frame: int
     return kv_num, kv_idx, full_num, full_idx
 
 
+# ---------------------------------------------------------------- paged cache
+@functools.lru_cache(maxsize=256)
+def _paged_geom(shape, stride, dtype, table_shape, table_stride) -> PagedGeom:
+    """Geometry of a page pool kv[2, P, Hkv, page, Dh] (any strides, head dim contiguous) with a table [S, M]."""
+    if len(shape) != 5 or shape[0] != 2 or stride[4] != 1:
+        raise ValueError("kv must be [2, pages, Hkv, page, Dh] with a contiguous last axis")
+    if len(table_shape) != 2 or table_stride[1] != 1:
+        raise ValueError("table must be [S, max_pages] with contiguous rows")
+    _, P, Hkv, page, Dh = shape
+    S, M = table_shape
+    return PagedGeom(S, Hkv, Dh, page, P, M, dtype_code(dtype), 0, stride[0], stride[1], stride[2], stride[3],
+                     table_stride[0])
+
+
+def _paged_check(kv, table, int32s, per_slot, others) -> PagedGeom:
+    """The checks every paged entry point makes: devices, types and shapes of the cache's tensors."""
+    device = kv.device
+    for t in (kv, table, *int32s, *per_slot, *others):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("world_engine_b200 runs on CUDA tensors only (sm_100a); there is no CPU path")
+        if t.device != device:
+            raise ValueError("all tensors of a paged cache call must be on the device of kv")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("the paged cache operators have no backward pass; call them under torch.no_grad()")
+    g = _paged_geom(kv.shape, kv.stride(), kv.dtype, table.shape, table.stride())
+    if table.dtype != torch.int32:
+        raise ValueError("table must be int32")
+    for t in int32s:
+        if t is not None and (t.dtype != torch.int32 or t.shape != (g.S, g.Hkv) or not t.is_contiguous()):
+            raise ValueError("token counts and positions must be contiguous int32 [S, Hkv]")
+    for t, dtype in zip(per_slot, (torch.float32, torch.int32)):
+        if t is not None and (t.dtype != dtype or t.shape != (g.n_pages, g.Hkv, g.page) or not t.is_contiguous()):
+            raise ValueError("weights (float32) and positions (int32) must be contiguous [pages, Hkv, page]")
+    return g
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return t.data_ptr() if t is not None else None
+
+
+def _call_on(device: torch.device, fn, args, where: str) -> None:
+    """One library call on the device of the tensors and its current stream."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(ctypes.byref(args), status_word(device).data_ptr(), _stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(ctypes.byref(args), status_word(device).data_ptr(), _stream_ptr(device))
+    _lib.check(rc, where)
+
+
+def _append_args(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new, lens_out,
+                 next_pos_out) -> PagedAppendArgs:
+    lens_out = lens if lens_out is None else lens_out
+    next_pos_out = next_pos if next_pos_out is None else next_pos_out
+    g = _paged_check(kv, table, (lens, next_pos, lens_out, next_pos_out), (weights, positions), (k_new, v_new, n_new, w_new))
+    S, Hkv, T, Dh = k_new.shape
+    if (S, Hkv, Dh) != (g.S, g.Hkv, g.Dh) or v_new.shape != k_new.shape or k_new.dtype != kv.dtype \
+            or v_new.dtype != kv.dtype:
+        raise ValueError("k_new and v_new must be [S, Hkv, T, Dh] of the cache's type")
+    if n_new is not None and (n_new.dtype != torch.int32 or n_new.shape != (S,) or not n_new.is_contiguous()):
+        raise ValueError("n_new must be contiguous int32 [S]")
+    if w_new is not None and (w_new.dtype != torch.float32 or w_new.shape != (S, Hkv, T)):
+        raise ValueError("w_new must be float32 [S, Hkv, T]")
+    return PagedAppendArgs(
+        g, k_new.data_ptr(), v_new.data_ptr(), _strides3(k_new), _strides3(v_new), kv.data_ptr(), _ptr(weights),
+        _ptr(positions), table.data_ptr(), lens.data_ptr(), next_pos.data_ptr(), lens_out.data_ptr(),
+        next_pos_out.data_ptr(), _ptr(n_new), _ptr(w_new),
+        Strides3(*w_new.stride()) if w_new is not None else Strides3(), None, 0, T, 0, 0, 0)
+
+
+def paged_append_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, next_pos: torch.Tensor,
+                  k_new: torch.Tensor, v_new: torch.Tensor, n_new: Optional[torch.Tensor] = None,
+                  weights: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                  w_new: Optional[torch.Tensor] = None, lens_out: Optional[torch.Tensor] = None,
+                  next_pos_out: Optional[torch.Tensor] = None) -> None:
+    """In-place append to a paged cache (we_b200_paged_append).  `kv [2, P, Hkv, page, Dh]` is the pool, row s of
+    `table [S, M]` the pages of session s, `lens` / `next_pos` `[S, Hkv]` the tokens a kv head holds and was ever
+    given.  `k_new` / `v_new` are `[S, Hkv, T, Dh]` views (any strides, head dim contiguous); of a padded batch only
+    the first `n_new[s]` tokens count.  The counts are updated in place unless `lens_out` / `next_pos_out` are
+    given.  Tokens for which a session has no room are dropped and reported by `check_status`."""
+    args = _append_args(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new, lens_out, next_pos_out)
+    _call_on(kv.device, _lib.load().we_b200_paged_append, args, "we_b200_paged_append")
+
+
+def paged_append_evict_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, next_pos: torch.Tensor,
+                        k_new: torch.Tensor, v_new: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor,
+                        keep: int, sink: int = 0, recent: int = 0, n_new: Optional[torch.Tensor] = None,
+                        w_new: Optional[torch.Tensor] = None, lens_out: Optional[torch.Tensor] = None,
+                        next_pos_out: Optional[torch.Tensor] = None) -> None:
+    """`paged_append_` under a budget (we_b200_paged_append_evict): afterwards no kv head holds more than `keep`
+    tokens.  Kept are the positions below `sink`, the last `recent` positions, and of the rest those with the
+    largest accumulated weight (of equal ones the lower index); tokens move only into the slots that evicted ones
+    left, so the order of a session's tokens is not kept (`positions` tells which is which)."""
+    if weights is None or positions is None:
+        raise ValueError("eviction needs weights and positions")
+    args = _append_args(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new, lens_out, next_pos_out)
+    args.keep, args.sink, args.recent = int(keep), int(sink), int(recent)
+    lib = _lib.load()
+    need = lib.we_b200_paged_evict_workspace_bytes(ctypes.byref(args.geom), args.T, args.keep)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=kv.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    _call_on(kv.device, lib.we_b200_paged_append_evict, args, "we_b200_paged_append_evict")
+
+
+def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float = 0.0,
+               weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+               lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per session over its paged cache (we_b200_paged_attn).  `q` is a
+    `[S, Hq, 1, Dh]` view; the output has its shape.  With `weights` the softmax weight every held token is given
+    (summed over the query heads of its kv head) is added to it in place; `lse` (float32 `[S, Hq]`, contiguous)
+    receives the logarithm of the softmax sum.  A kv head that holds nothing gives 0 and -inf."""
+    g = _paged_check(kv, table, (lens,), (weights,), (q, out, lse))
+    S, Hq, T, Dh = q.shape
+    if (S, T, Dh) != (g.S, 1, g.Dh) or q.dtype != kv.dtype or q.stride(3) != 1:
+        raise ValueError("q must be [S, Hq, 1, Dh] of the cache's type with a contiguous last axis")
+    if out is None:
+        out = torch.empty((S, Hq, 1, Dh), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
+        raise ValueError("out must have q's shape and type and a contiguous last axis")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (S, Hq) or not lse.is_contiguous()):
+        raise ValueError("lse must be contiguous float32 [S, Hq]")
+    lib = _lib.load()
+    need = lib.we_b200_paged_attn_workspace_bytes(ctypes.byref(g), Hq, weights is not None)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    qs, os_ = q.stride(), out.stride()
+    args = PagedAttnArgs(g, q.data_ptr(), out.data_ptr(), (qs[0], qs[1]), (os_[0], os_[1]), kv.data_ptr(),
+                         table.data_ptr(), lens.data_ptr(), _ptr(weights), _ptr(lse), _ptr(ws), need, Hq, scale)
+    _call_on(q.device, lib.we_b200_paged_attn, args, "we_b200_paged_attn")
+    return out
+
+
 # ----------------------------------------------------------------- custom ops
 # Registered under the reference's own namespace style ("world_engine::...").
 @torch.library.custom_op("world_engine_b200::append_attend", mutates_args=("kv", "written"))
@@ -329,3 +465,42 @@ def append_attend_gated_op(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Te
 def _append_attend_gated_fake(q, k_new, v_new, kv, written, frame_t, gate, tokens_per_frame, dilation, is_frozen,
                               scale, gate_is_logits):
     return torch.empty_like(q)
+
+
+@torch.library.custom_op("world_engine_b200::paged_append",
+                         mutates_args=("kv", "lens", "next_pos", "weights", "positions"))
+def paged_append_op(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, next_pos: torch.Tensor,
+                    k_new: torch.Tensor, v_new: torch.Tensor, n_new: Optional[torch.Tensor], weights: torch.Tensor,
+                    positions: torch.Tensor, w_new: Optional[torch.Tensor]) -> None:
+    paged_append_(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new)
+
+
+@paged_append_op.register_fake
+def _paged_append_fake(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new):
+    return None
+
+
+@torch.library.custom_op("world_engine_b200::paged_append_evict",
+                         mutates_args=("kv", "lens", "next_pos", "weights", "positions"))
+def paged_append_evict_op(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, next_pos: torch.Tensor,
+                          k_new: torch.Tensor, v_new: torch.Tensor, weights: torch.Tensor, positions: torch.Tensor,
+                          keep: int, sink: int, recent: int, n_new: Optional[torch.Tensor],
+                          w_new: Optional[torch.Tensor]) -> None:
+    paged_append_evict_(kv, table, lens, next_pos, k_new, v_new, weights, positions, keep, sink, recent, n_new, w_new)
+
+
+@paged_append_evict_op.register_fake
+def _paged_append_evict_fake(kv, table, lens, next_pos, k_new, v_new, weights, positions, keep, sink, recent, n_new,
+                             w_new):
+    return None
+
+
+@torch.library.custom_op("world_engine_b200::paged_attn", mutates_args=("weights",))
+def paged_attn_op(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float,
+                  weights: Optional[torch.Tensor]) -> torch.Tensor:
+    return paged_attn(q, kv, table, lens, scale, weights)
+
+
+@paged_attn_op.register_fake
+def _paged_attn_fake(q, kv, table, lens, scale, weights):
+    return q.new_empty(q.shape)
