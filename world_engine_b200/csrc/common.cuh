@@ -64,6 +64,10 @@ __host__ __device__ inline SlotInfo slot_of(int64_t frame_t, int64_t L, int T, i
   return s;
 }
 
+// SMs of the current device.
+constexpr int kMaxDevices = 64;
+int sm_count();
+
 int kv_append_launch(const void* k_new, const int64_t* ks, const void* v_new, const int64_t* vs, void* kv,
                      uint8_t* written, uint8_t* mask_written, const int64_t* frame_t, const we_b200_cache_geom* g,
                      int is_frozen, cudaStream_t stream);

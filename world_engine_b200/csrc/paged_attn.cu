@@ -1,114 +1,876 @@
 // Attention of one new token per session over the paged KV cache (sm_100a).
+//
+//   x_gj = scale q_g . k_j,   p_gj = 2^(x_gj log2 e - m_g) / l_g,   o_g = sum_j p_gj v_j,   weight_j += sum_g p_gj
+//
+// Every K and V row is used for the few query heads that share its kv head, once: the work is reading the cache, and
+// the kernel is built so that nothing but TMA touches it on the way to the tensor cores.  The products are turned
+// around: 128 tokens are the M rows of S^T = K Q^T and the head dim is M of O^T = V^T P^T, the query heads are the N
+// columns, so K (K-major) and V (MN-major) are read as they lie in shared memory.
+//
+// Work is cut by tokens, not by heads: the tokens of all (session, kv head, chunk of 16 query heads) units are laid end
+// to end in granules of 16 or 32 tokens and every CTA gets an equal run of them, whatever the sessions' lengths, so
+// all SMs finish together.  A run crosses units: each piece is a segment, with its own softmax statistics.  A unit that
+// lies in one CTA is finished there; of one that several CTAs share each leaves (m, l, O) in the workspace and
+// paged_join_kernel puts them together, in the order of the tokens.
+//
+// One CTA per SM, 256 threads:
+//   warps 0-3  softmax.  Thread t owns token t of a tile (TMEM lane t): its logits of the G heads are G columns.  The
+//              reference m_g is raised only when a logit exceeds it by more than 8 (then O is rescaled in tensor
+//              memory), so a tile costs one vote among the 128 threads and no reduction.  P goes to shared memory as
+//              the sum of two 16-bit numbers in two columns: the second column costs nothing (N is at least 16) and
+//              leaves the weights accurate to 2^-16 instead of 2^-8.
+//   warp 4     K: walks the run, publishes the segments with their Q rows, loads the K tiles
+//   warp 7     V tiles (a ring of its own)
+//   warp 5     issues S^T, warp 6 issues O^T (one thread each)
+// Tensor memory (64 columns): S0, S1 (16 each), O (high and low parts of up to 16 heads: 32).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
 
 #include "paged.cuh"
+#include "ptx.cuh"
 
 namespace we {
 
 constexpr int kPagedThreads = 256;
+constexpr int kTile = 128;                 // tokens per tile
+constexpr int kSegs = 4;                   // segments in flight
+constexpr int kMaxGroup = 16;              // query heads per unit
+constexpr float kRaise = 8.0f;             // log2 units by which a logit may exceed the reference
+constexpr int kJoinThreads = 256;
+constexpr int kWholeUnitTokens = 128;      // sessions this short are never split
 
 struct PagedAttnParams {
   PagedView v;
   const uint16_t* q;
   uint16_t* out;
   int64_t qs[2], os[2];
-  const uint16_t* kv;
   const int32_t* lens;
   float* weights;
   float* lse;
-  int32_t Hq, group;
+  // workspace
+  int32_t* ws_prefix;        // [units + 1] granules before a unit
+  float2* ws_ml;             // [2 grid][GP] statistics of the segments of shared units
+  float* ws_o;               // [2 grid][GP][DH]
+  float* ws_lse;             // [units][GP] log2 of the softmax sum of units one CTA finished
+  float* ws_x;               // [units][GP][cap] logits (log2 units)
+  int64_t x_stride;          // max_pages * page
+  int64_t unit_plane, unit_page, unit_head;   // tensor map coordinates of the V plane, of a page, of a head
+  int32_t Hq, group, chunks; // query heads, per kv head, units per kv head
+  int32_t units, grid;
+  int32_t gran_shift;        // log2 of the tokens per granule
+  int32_t whole;             // 1: every unit belongs to one CTA (no join)
+  int32_t min_share;         // granules a CTA gets at least
   float scale_log2;
 };
 
+struct Segment {
+  int32_t unit, tok0, ntok;  // ntok 0: the end of the run
+  int32_t slot;              // workspace slot, or -1: the segment is the whole unit
+};
+
 template <bool BF16>
-__device__ __forceinline__ float to_float(uint16_t x) {
-  if constexpr (BF16) return __bfloat162float(__ushort_as_bfloat16(x));
-  else return __half2float(__ushort_as_half(x));
-}
-template <bool BF16>
-__device__ __forceinline__ uint16_t from_float(float x) {
+__device__ __forceinline__ uint16_t narrow(float x) {
   if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
   else return __half_as_ushort(__float2half_rn(x));
 }
+template <bool BF16>
+__device__ __forceinline__ float widen(uint16_t x) {
+  if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(x) << 16);
+  else return __half2float(__ushort_as_half(x));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+__device__ __forceinline__ bool bar_any(int id, int n, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 q, %3, 0;\n\t"
+      "bar.red.or.pred p, %1, %2, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"(id), "r"(n), "r"(x ? 1u : 0u)
+      : "memory");
+  return r != 0;
+}
 
-template <bool BF16, int DH>
-__global__ void __launch_bounds__(kPagedThreads) paged_attn_kernel(const PagedAttnParams p) {
+template <int DH, int GP>
+struct PagedCfg {
+  static constexpr int kChunks = DH / 64;
+  static constexpr int kRowGroup = kChunks * 1024;           // 8 tokens: [chunk][8 rows][128 bytes]
+  static constexpr int kTileBytes = 16 * kRowGroup;
+  static constexpr int kStages = DH == 128 ? 3 : 6;
+  static constexpr int kNP = 2 * GP <= 16 ? 16 : 32;         // columns of O^T
+  static constexpr int kQBytes = 16 * DH * 2;                // [chunk][16 rows][128 bytes]
+  static constexpr int kPBytes = 2 * kNP * 128;              // [64 tokens][kNP rows][128 bytes]
+  static constexpr int kOffV = kStages * kTileBytes;
+  static constexpr int kOffQ = 2 * kStages * kTileBytes;
+  static constexpr int kOffP = kOffQ + kSegs * kQBytes;
+  static constexpr int kOffAux = kOffP + 2 * kPBytes;
+  static constexpr int kAux = 512 + 2 * 4 * 16 * 4 + 64 + 64;
+  static constexpr int kSmem = kOffAux + kAux + 1024;
+};
+
+// The heads of a unit.
+struct UnitHeads {
+  int s, h, hq0, n;          // session, kv head, first query head, query heads
+};
+__device__ __forceinline__ UnitHeads unit_heads(const PagedAttnParams& p, int u) {
+  UnitHeads r;
+  const int sh = u / p.chunks, c = u - sh * p.chunks;
+  r.s = sh / p.v.Hkv;
+  r.h = sh - r.s * p.v.Hkv;
+  r.hq0 = r.h * p.group + c * kMaxGroup;
+  r.n = min(p.group - c * kMaxGroup, kMaxGroup);
+  return r;
+}
+
+// A unit that holds nothing.
+__device__ void write_empty(const PagedAttnParams& p, int u, int dh) {
+  const UnitHeads w = unit_heads(p, u);
+  for (int g = 0; g < w.n; ++g) {
+    uint4* dst = reinterpret_cast<uint4*>(p.out + w.s * p.os[0] + (w.hq0 + g) * p.os[1]);
+    for (int i = 0; i < dh / 8; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (p.lse != nullptr) p.lse[static_cast<int64_t>(w.s) * p.Hq + w.hq0 + g] = -INFINITY;
+  }
+}
+
+__device__ __forceinline__ int share_of(const PagedAttnParams& p, int total) {
+  return max((total + p.grid - 1) / p.grid, p.min_share);
+}
+
+template <int DH, bool BF16, int GP>
+__global__ void __launch_bounds__(kPagedThreads, 1)
+paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams p) {
+  using C = PagedCfg<DH, GP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* sK = smem;
+  uint8_t* sV = smem + C::kOffV;
+  uint8_t* sQ = smem + C::kOffQ;
+  uint8_t* sP = smem + C::kOffP;
+  uint8_t* aux = smem + C::kOffAux;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(aux);
+  uint64_t* k_empty = k_full + C::kStages;
+  uint64_t* v_full = k_empty + C::kStages;
+  uint64_t* v_empty = v_full + C::kStages;
+  uint64_t* q_full = v_empty + C::kStages;
+  uint64_t* q_empty = q_full + kSegs;
+  uint64_t* s_full = q_empty + kSegs;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* pv_done = p_full + 2;
+  float* s_max = reinterpret_cast<float*>(aux + 512);                 // [4 warps][16]
+  float* s_sum = s_max + 64;                                          // [4 warps][16]
+  Segment* segs = reinterpret_cast<Segment*>(aux + 1024);
+  int* s_plan = reinterpret_cast<int*>(aux + 1024 + kSegs * 16);      // 0 unit, 1 granule, 2 run, 4.. scan
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_plan + 14);
+  volatile int* s_abort = s_plan + 15;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+  if (warp == 5) {
+    tmem_alloc(s_tmem, 64);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < kSegs; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 7);         // four softmax warps, both issuers, the V producer
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&pv_done[i], 1);
+    }
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (tid == 128) prefetch_tensormap(&tm);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kWarps = kPagedThreads / 32, kPer = DH / 32;
-  __shared__ float s_m[kWarps], s_l[kWarps], s_o[kWarps][DH];
-  const int h = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int len = paged_count(p.v, p.lens[s * p.v.Hkv + h]);
-  for (int g = 0; g < p.group; ++g) {
-    const int hq = h * p.group + g;
-    float q[kPer], o[kPer];
-    for (int u = 0; u < kPer; ++u) {
-      q[u] = to_float<BF16>(p.q[s * p.qs[0] + hq * p.qs[1] + kPer * lane + u]);
-      o[u] = 0.f;
+
+  // ------------------------------------------------------------------ this CTA's run of granules
+  auto held = [&](int u) { return paged_count(p.v, p.lens[u / p.chunks]); };
+  const int gs = p.gran_shift;
+  auto granules = [&](int n) { return (n + (1 << gs) - 1) >> gs; };
+  int end_unit = p.units;
+  if (p.whole) {
+    const int u0 = static_cast<int>(static_cast<int64_t>(p.units) * cta / p.grid);
+    end_unit = static_cast<int>(static_cast<int64_t>(p.units) * (cta + 1) / p.grid);
+    if (tid == 0) {
+      s_plan[0] = u0;
+      s_plan[1] = 0;
+      s_plan[2] = 0x7FFFFFFF;
     }
-    float m = -INFINITY, l = 0.f;
-    auto row_of = [&](int j) {
-      int pg = paged_page(p.v, s, j >> p.v.page_shift);
-      if (pg < 0) pg = 0;
-      return p.kv + pg * p.v.page_s + h * p.v.head_s + (j & (p.v.page - 1)) * p.v.token_s + kPer * lane;
-    };
-    auto score = [&](const uint16_t* k) {
-      float x = 0.f;
-      for (int u = 0; u < kPer; ++u) x = fmaf(q[u], to_float<BF16>(k[u]), x);
-      for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-      return x * p.scale_log2;
-    };
-    for (int j = wid; j < len; j += kWarps) {
-      const uint16_t* k = row_of(j);
-      const float x = score(k);
-      const float mn = fmaxf(m, x);
-      const float a = mn == m ? 1.f : exp2f(m - mn), w = exp2f(x - mn);
-      l = l * a + w;
-      for (int u = 0; u < kPer; ++u) o[u] = o[u] * a + w * to_float<BF16>(k[p.v.plane_s + u]);
-      m = mn;
+    for (int u = u0 + tid; u < end_unit; u += kPagedThreads)
+      if (held(u) == 0) write_empty(p, u, DH);
+  } else {
+    const int per = (p.units + kPagedThreads - 1) / kPagedThreads;
+    const int first = min(tid * per, p.units), last = min(first + per, p.units);
+    int sum = 0;
+    for (int u = first; u < last; ++u) {
+      const int n = held(u);
+      sum += granules(n);
+      if (n == 0 && u % p.grid == cta) write_empty(p, u, DH);
     }
+    int pre = sum;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, pre, d);
+      if (lane >= d) pre += y;
+    }
+    if (lane == 31) s_plan[4 + warp] = pre;
     __syncthreads();
-    if (lane == 0) s_m[wid] = m, s_l[wid] = l;
-    for (int u = 0; u < kPer; ++u) s_o[wid][kPer * lane + u] = o[u];
-    __syncthreads();
-    float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w]);
-    for (int w = 0; w < kWarps && w < len; ++w) sum += s_m[w] == top ? s_l[w] : s_l[w] * exp2f(s_m[w] - top);
-    const float lse2 = top + log2f(sum);
-    for (int d = threadIdx.x; d < DH; d += kPagedThreads) {
-      float x = 0.f;
-      for (int w = 0; w < kWarps && w < len; ++w) x += s_m[w] == top ? s_o[w][d] : s_o[w][d] * exp2f(s_m[w] - top);
-      p.out[s * p.os[0] + hq * p.os[1] + d] = from_float<BF16>(len > 0 ? x / sum : 0.f);
+    int total = 0;
+    for (int w = 0; w < kPagedThreads / 32; ++w) {
+      const int y = s_plan[4 + w];
+      if (w < warp) pre += y;
+      total += y;
     }
-    if (threadIdx.x == 0 && p.lse != nullptr) p.lse[s * p.Hq + hq] = len > 0 ? lse2 * 0.6931471805599453f : -INFINITY;
-    if (p.weights != nullptr) {
-      for (int j = wid; j < len; j += kWarps) {
-        const float x = score(row_of(j));
-        const int pg = paged_page(p.v, s, j >> p.v.page_shift);
-        if (lane == 0 && pg >= 0)
-          atomicAdd(p.weights + (static_cast<int64_t>(pg) * p.v.Hkv + h) * p.v.page + (j & (p.v.page - 1)), exp2f(x - top) / sum);
+    pre -= sum;
+    const int share = share_of(p, total);
+    const int64_t g0 = static_cast<int64_t>(share) * cta;
+    const int run = g0 < total ? static_cast<int>(min(static_cast<int64_t>(share), total - g0)) : 0;
+    if (tid == 0) s_plan[2] = run;
+    if (run > 0 && g0 >= pre && g0 < pre + sum) {
+      int u = first, at = pre;
+      for (int n = granules(held(u)); at + n <= g0; n = granules(held(++u))) at += n;
+      s_plan[0] = u;
+      s_plan[1] = static_cast<int>(g0) - at;
+    }
+    if (cta == 0) {                      // for the join
+      int at = pre;
+      for (int u = first; u < last; ++u) {
+        p.ws_prefix[u] = at;
+        at += granules(held(u));
+      }
+      if (tid == 0) p.ws_prefix[p.units] = total;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = *s_tmem;
+  constexpr uint32_t kColO = 32;
+
+  if (warp == 4) {
+    // ---------------------------------------------------------------- K tiles and segments
+    int u = s_plan[0], at = s_plan[1], left = s_plan[2];
+    int seg = 0, it = 0;
+    bool ok = true;
+    while (ok && left > 0 && u < end_unit) {
+      const int n = held(u), tok0 = at << gs;
+      int ntok = n - tok0;
+      if (!p.whole) ntok = static_cast<int>(min(static_cast<int64_t>(ntok), static_cast<int64_t>(left) << gs));
+      if (ntok <= 0) {
+        ++u;
+        at = 0;
+        continue;
+      }
+      const UnitHeads w = unit_heads(p, u);
+      const int qslot = seg % kSegs, end = tok0 + ntok, x0 = w.h * static_cast<int>(p.unit_head);
+      auto page_at = [&](int tok) {
+        if (lane >= (kTile >> gs) || tok >= end) return -1;
+        const int pg = paged_page(p.v, w.s, tok >> p.v.page_shift);
+        return pg < 0 ? 0 : pg;
+      };
+      int tok = tok0 + (lane << gs), pg = page_at(tok);
+      constexpr int kVecs = DH / 8, kLoads = (GP * kVecs + 31) / 32;
+      uint4 q[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int e = lane + 32 * i, row = e / kVecs, vec = e % kVecs;
+        q[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < w.n && row < GP)
+          q[i] = *reinterpret_cast<const uint4*>(p.q + w.s * p.qs[0] + (w.hq0 + row) * p.qs[1] + 8 * vec);
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qslot], ((seg / kSegs) & 1) ^ 1, s_abort));
+      for (int t0 = tok0; t0 < end && ok; t0 += kTile, ++it) {
+        const int st = it % C::kStages, ng = (min(kTile, end - t0) + (1 << gs) - 1) >> gs;
+        const int next = tok + kTile, pg_next = page_at(next);
+        ok = mbar_wait(&k_empty[st], ((it / C::kStages) & 1) ^ 1, s_abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&k_full[st], (ng << gs) * DH * 2);
+        __syncwarp();
+        if (lane < ng)
+          tma_load_5d(smem_u32(sK + st * C::kTileBytes) + lane * ((DH * 2) << gs), &tm, &k_full[st], 0, 0, 0,
+                      (tok & (p.v.page - 1)) >> 3, pg * static_cast<int>(p.unit_page) + x0);
+        tok = next;
+        pg = pg_next;
+        if (t0 == tok0) {
+          // the segment's query rows: [chunk][16 rows][128 bytes], 128-byte swizzle
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) {
+            const int e = lane + 32 * i, row = e / kVecs, vec = e % kVecs;
+            if (row < GP)
+              *reinterpret_cast<uint4*>(sQ + qslot * C::kQBytes + (vec >> 3) * 2048 + row * 128 +
+                                        (((vec & 7) ^ (row & 7)) << 4)) = q[i];
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            Segment d;
+            d.unit = u;
+            d.tok0 = tok0;
+            d.ntok = ntok;
+            d.slot = (tok0 == 0 && ntok == n) ? -1 : 2 * cta + (seg == 0 ? 0 : 1);
+            segs[qslot] = d;
+            mbar_arrive(&q_full[qslot]);
+          }
+        }
+      }
+      ++seg;
+      if (!p.whole) left -= granules(ntok);
+      ++u;
+      at = 0;
+    }
+    if (ok && mbar_wait(&q_empty[seg % kSegs], ((seg / kSegs) & 1) ^ 1, s_abort) && lane == 0) {
+      segs[seg % kSegs].ntok = 0;
+      mbar_arrive(&q_full[seg % kSegs]);
+    }
+  } else if (warp == 7) {
+    // ---------------------------------------------------------------- V tiles
+    int it = 0;
+    for (int seg = 0;; ++seg) {
+      const int qslot = seg % kSegs;
+      bool ok = mbar_wait(&q_full[qslot], (seg / kSegs) & 1, s_abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const Segment d = segs[qslot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[qslot]);
+      if (d.ntok == 0) break;
+      const UnitHeads w = unit_heads(p, d.unit);
+      const int end = d.tok0 + d.ntok, x0 = w.h * static_cast<int>(p.unit_head) + static_cast<int>(p.unit_plane);
+      auto page_at = [&](int tok) {
+        if (lane >= (kTile >> gs) || tok >= end) return -1;
+        const int pg = paged_page(p.v, w.s, tok >> p.v.page_shift);
+        return pg < 0 ? 0 : pg;
+      };
+      int tok = d.tok0 + (lane << gs), pg = page_at(tok);
+      for (int t0 = d.tok0; t0 < end; t0 += kTile, ++it) {
+        const int st = it % C::kStages, ng = (min(kTile, end - t0) + (1 << gs) - 1) >> gs;
+        const int next = tok + kTile, pg_next = page_at(next);
+        ok = mbar_wait(&v_empty[st], ((it / C::kStages) & 1) ^ 1, s_abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) mbar_arrive_expect_tx(&v_full[st], (ng << gs) * DH * 2);
+        __syncwarp();
+        if (lane < ng)
+          tma_load_5d(smem_u32(sV + st * C::kTileBytes) + lane * ((DH * 2) << gs), &tm, &v_full[st], 0, 0, 0,
+                      (tok & (p.v.page - 1)) >> 3, pg * static_cast<int>(p.unit_page) + x0);
+        tok = next;
+        pg = pg_next;
       }
     }
+  } else if (warp == 5) {
+    // ---------------------------------------------------------------- S^T = K Q^T: 128 tokens x 16 heads
+    if (lane == 0) {
+      constexpr uint32_t kIdesc = umma_idesc(BF16 ? 1u : 0u, 0u, kTile, 16);
+      constexpr uint32_t kHiK = umma_desc_hi(C::kRowGroup), kHiQ = umma_desc_hi(1024);
+      int it = 0;
+      bool ok = true;
+      for (int seg = 0; ok; ++seg) {
+        const int qslot = seg % kSegs;
+        if (!mbar_wait(&q_full[qslot], (seg / kSegs) & 1, s_abort)) break;
+        const int ntok = segs[qslot].ntok;
+        if (ntok == 0) break;
+        const uint32_t q_lo = umma_desc_lo(smem_u32(sQ + qslot * C::kQBytes), 16);
+        for (int t0 = 0; t0 < ntok && ok; t0 += kTile, ++it) {
+          const int st = it % C::kStages;
+          ok = mbar_wait(&k_full[st], (it / C::kStages) & 1, s_abort);
+          if (it >= 2) ok = mbar_wait(&p_full[it & 1], ((it - 2) >> 1) & 1, s_abort) && ok;    // S(it - 2) was read
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t k_lo = umma_desc_lo(smem_u32(sK + st * C::kTileBytes), 16);
+#pragma unroll
+          for (int kk = 0; kk < DH / 16; ++kk)
+            umma_ss(tmem + 16 * (it & 1), k_lo + (kk >> 2) * 64 + (kk & 3) * 2, kHiK, q_lo + (kk >> 2) * 128 + (kk & 3) * 2,
+                    kHiQ, kIdesc, kk > 0);
+          tc_commit(&s_full[it & 1]);
+          tc_commit(&k_empty[st]);
+        }
+        tc_commit(&q_empty[qslot]);
+      }
+    }
+  } else if (warp == 6) {
+    // ---------------------------------------------------------------- O^T += V^T P^T: 128 rows (of the head dim) x heads
+    if (lane == 0) {
+      constexpr uint32_t kIdesc = umma_idesc(BF16 ? 1u : 0u, 0u, 128, C::kNP) | (1u << 15);     // A is MN-major
+      constexpr uint32_t kHiV = umma_desc_hi(C::kRowGroup), kHiP = umma_desc_hi(1024);
+      int it = 0;
+      bool ok = true;
+      for (int seg = 0; ok; ++seg) {
+        const int qslot = seg % kSegs;
+        if (!mbar_wait(&q_full[qslot], (seg / kSegs) & 1, s_abort)) break;
+        const int ntok = segs[qslot].ntok;
+        mbar_arrive(&q_empty[qslot]);
+        if (ntok == 0) break;
+        for (int t0 = 0; t0 < ntok && ok; t0 += kTile, ++it) {
+          const int st = it % C::kStages, steps = (min(kTile, ntok - t0) + 15) >> 4;
+          ok = mbar_wait(&v_full[st], (it / C::kStages) & 1, s_abort);
+          ok = mbar_wait(&p_full[it & 1], (it >> 1) & 1, s_abort) && ok;
+          if (!ok) break;
+          tc_fence_after();
+          // (head dim 64: rows 64.. of the product read the next eight tokens in place of a second column chunk;
+          // nobody reads what they give)
+          const uint32_t v_lo = umma_desc_lo(smem_u32(sV + st * C::kTileBytes), 1024);
+          const uint32_t p_lo = umma_desc_lo(smem_u32(sP + (it & 1) * C::kPBytes), 16);
+          for (int kk = 0; kk < steps; ++kk)
+            umma_ss(tmem + kColO, v_lo + kk * (2 * C::kRowGroup >> 4), kHiV, p_lo + (kk >> 2) * (C::kNP * 128 >> 4) + (kk & 3) * 2,
+                    kHiP, kIdesc, t0 > 0 || kk > 0);
+          tc_commit(&v_empty[st]);
+          tc_commit(&pv_done[it & 1]);
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    int it = 0;
+    for (int seg = 0;; ++seg) {
+      const int qslot = seg % kSegs;
+      const bool ok = mbar_wait(&q_full[qslot], (seg / kSegs) & 1, s_abort);
+      __syncwarp();
+      if (bar_any(1, 128, !ok)) break;
+      const Segment d = segs[qslot];
+      if (d.ntok == 0) break;
+      const UnitHeads w = unit_heads(p, d.unit);
+      float m[GP], l[GP];
+#pragma unroll
+      for (int g = 0; g < GP; ++g) m[g] = -INFINITY, l[g] = 0.f;
+      float* xs = p.weights != nullptr ? p.ws_x + static_cast<int64_t>(d.unit) * GP * p.x_stride + d.tok0 : nullptr;
+      for (int t0 = 0; t0 < d.ntok; t0 += kTile, ++it) {
+        const int buf = it & 1, nv = min(kTile, d.ntok - t0);
+        mbar_wait(&s_full[buf], (it >> 1) & 1, s_abort);
+        __syncwarp();
+        tc_fence_after();
+        uint32_t raw[GP];
+        tmem_ld_n<GP>(tmem + lanes + 16 * buf, raw);
+        tmem_ld_wait();
+        float x[GP];
+        bool raise = false;
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          x[g] = tid < nv && g < w.n ? __uint_as_float(raw[g]) * p.scale_log2 : -INFINITY;
+          raise |= x[g] > m[g] + kRaise;
+        }
+        if (xs != nullptr && tid < nv) {
+#pragma unroll
+          for (int g = 0; g < GP; ++g)
+            if (g < w.n) xs[g * p.x_stride + t0 + tid] = x[g];
+        }
+        if (bar_any(1, 128, raise)) {
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            float t = x[g];
+            for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            if (lane == 0) s_max[warp * 16 + g] = t;
+          }
+          bar_sync(1, 128);
+          float f[GP];
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            const float t = fmaxf(fmaxf(fmaxf(s_max[g], s_max[16 + g]), fmaxf(s_max[32 + g], s_max[48 + g])), m[g]);
+            f[g] = t == m[g] ? 1.f : exp2_fast(m[g] - t);
+            m[g] = t;
+            l[g] *= f[g];
+          }
+          if (t0 > 0) {
+            mbar_wait(&pv_done[buf ^ 1], ((it - 1) >> 1) & 1, s_abort);
+            __syncwarp();
+            tc_fence_after();
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              uint32_t o[GP];
+              tmem_ld_n<GP>(tmem + lanes + kColO + part * GP, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int g = 0; g < GP; ++g) o[g] = __float_as_uint(__uint_as_float(o[g]) * f[g]);
+              tmem_st_n<GP>(tmem + lanes + kColO + part * GP, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        if (it >= 2) mbar_wait(&pv_done[buf], ((it - 2) >> 1) & 1, s_abort);      // P(it - 2) was read
+        uint8_t* pw = sP + buf * C::kPBytes + (tid >> 6) * (C::kNP * 128);
+        const uint32_t col = (tid & 63) * 2;
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          const float e = exp2_fast(x[g] - (m[g] == -INFINITY ? 0.f : m[g]));
+          l[g] += e;
+          const uint16_t hi = narrow<BF16>(e);
+          const uint16_t lo = narrow<BF16>(e - widen<BF16>(hi));
+          *reinterpret_cast<uint16_t*>(pw + g * 128 + (col ^ ((g & 7) << 4))) = hi;
+          *reinterpret_cast<uint16_t*>(pw + (GP + g) * 128 + (col ^ (((GP + g) & 7) << 4))) = lo;
+        }
+        if (tid >= nv && tid < ((nv + 15) & ~15)) {
+          // rows behind the last token: whatever the page holds there must not meet a weight of zero
+          const int st = it % C::kStages;
+          mbar_wait(&v_full[st], (it / C::kStages) & 1, s_abort);
+          uint8_t* row = sV + st * C::kTileBytes + (tid >> 3) * C::kRowGroup + (tid & 7) * 128;
+#pragma unroll
+          for (int c = 0; c < C::kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(row + c * 1024 + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(&p_full[buf]);
+      }
+      // ---- the segment's sums
+#pragma unroll
+      for (int g = 0; g < GP; ++g) {
+        for (int o = 16; o > 0; o >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
+        if (lane == 0) s_sum[warp * 16 + g] = l[g];
+      }
+      bar_sync(1, 128);
+#pragma unroll
+      for (int g = 0; g < GP; ++g) l[g] = (s_sum[g] + s_sum[16 + g]) + (s_sum[32 + g] + s_sum[48 + g]);
+      mbar_wait(&pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, s_abort);
+      __syncwarp();
+      tc_fence_after();
+      uint32_t hi[GP], lo[GP];
+      tmem_ld_n<GP>(tmem + lanes + kColO, hi);
+      tmem_ld_n<GP>(tmem + lanes + kColO + GP, lo);
+      tmem_ld_wait();
+      float o[GP];
+#pragma unroll
+      for (int g = 0; g < GP; ++g) {
+        // (an infinite value times a low part, which may be 0 or negative, is none of the formula's terms)
+        const float y = __uint_as_float(lo[g]);
+        o[g] = __uint_as_float(hi[g]) + (fabsf(y) < INFINITY ? y : 0.f);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_empty[qslot]);
+      if (d.slot >= 0) {
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          if (g >= w.n) continue;
+          if (tid < DH)
+            p.ws_o[(static_cast<int64_t>(d.slot) * GP + g) * DH + tid] = o[g];
+          if (tid == g) p.ws_ml[d.slot * GP + g] = make_float2(m[g], l[g]);
+        }
+        continue;
+      }
+      float lse[GP];
+#pragma unroll
+      for (int g = 0; g < GP; ++g) {
+        lse[g] = m[g] + log2f(l[g]);
+        if (g >= w.n) continue;
+        if (tid < DH)
+          p.out[w.s * p.os[0] + (w.hq0 + g) * p.os[1] + tid] = narrow<BF16>(o[g] / l[g]);
+        if (tid == g) {
+          if (p.lse != nullptr) p.lse[static_cast<int64_t>(w.s) * p.Hq + w.hq0 + g] = lse[g] * 0.6931471805599453f;
+          if (xs != nullptr) p.ws_lse[static_cast<int64_t>(d.unit) * GP + g] = lse[g];
+        }
+      }
+      if (xs != nullptr && p.chunks == 1) {
+        for (int t = tid; t < d.ntok; t += 128) {                     // (d.tok0 is 0)
+          float add = 0.f;
+#pragma unroll
+          for (int g = 0; g < GP; ++g)
+            if (g < w.n) add += exp2_fast(xs[g * p.x_stride + t] - lse[g]);
+          const int pg = paged_page(p.v, w.s, t >> p.v.page_shift);
+          if (pg >= 0)
+            atomicAdd(p.weights + (static_cast<int64_t>(pg) * p.v.Hkv + w.h) * p.v.page + (t & (p.v.page - 1)), add);
+        }
+      }
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  tc_fence_before();
+  __syncthreads();
+  if (*s_abort != 0) {
+    if (tid == 0 && p.v.status != nullptr) atomicExch(p.v.status, WE_B200_ST_WAIT_EXPIRED);
+    __nanosleep(1000000);  // let copies and products that are still in flight land before the CTA goes away
     __syncthreads();
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 64);
+  }
+}
+
+// ------------------------------------------------------------------ units that several CTAs share
+// Where the pieces of a unit lie: CTA c0 .. c1, and the workspace slot of each.
+struct Pieces {
+  int c0, n, slot0;
+};
+__device__ __forceinline__ Pieces pieces_of(int a, int b, int share) {
+  Pieces r;
+  r.c0 = a / share;
+  r.n = (b - 1) / share - r.c0 + 1;
+  r.slot0 = 2 * r.c0 + (a == r.c0 * share ? 0 : 1);
+  return r;
+}
+__device__ __forceinline__ int slot_of_piece(const Pieces& r, int k) { return k == 0 ? r.slot0 : 2 * (r.c0 + k); }
+
+// Softmax statistics of a head over the pieces of its unit, by one warp: maximum and sum, in every lane.
+template <int GP>
+__device__ __forceinline__ float2 join_ml(const PagedAttnParams& p, const Pieces& r, int g, int lane) {
+  float top = -INFINITY;
+  for (int k = lane; k < r.n; k += 32) top = fmaxf(top, p.ws_ml[slot_of_piece(r, k) * GP + g].x);
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f;
+  for (int k = lane; k < r.n; k += 32) {
+    const float2 ml = p.ws_ml[slot_of_piece(r, k) * GP + g];
+    sum += ml.y * exp2_fast(ml.x - top);
+  }
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return make_float2(top, sum);
+}
+
+template <int DH, bool BF16, int GP>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int kWarps = kJoinThreads / 32, kPer = DH / 32;
+  __shared__ float s_o[kWarps][DH];
+  __shared__ float s_lse[kMaxGroup];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int total = p.ws_prefix[p.units], share = share_of(p, total);
+  // ---- outputs: one head at a time
+  const int heads = min(p.group, kMaxGroup);
+  for (int64_t item = blockIdx.x; item < static_cast<int64_t>(p.units) * heads; item += gridDim.x) {
+    const int u = static_cast<int>(item / heads), g = static_cast<int>(item - static_cast<int64_t>(u) * heads);
+    const int a = p.ws_prefix[u], b = p.ws_prefix[u + 1];
+    if (a == b) continue;
+    const Pieces r = pieces_of(a, b, share);
+    const UnitHeads w = unit_heads(p, u);
+    if (r.n == 1 || g >= w.n) continue;
+    const float2 ml = join_ml<GP>(p, r, g, lane);
+    float o[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] = 0.f;
+    for (int k = warp; k < r.n; k += kWarps) {
+      const int64_t at = static_cast<int64_t>(slot_of_piece(r, k)) * GP + g;
+      const float f = exp2_fast(p.ws_ml[at].x - ml.x);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) o[i] += f * p.ws_o[at * DH + 32 * i + lane];
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s_o[warp][32 * i + lane] = o[i];
+    __syncthreads();
+    if (tid < DH) {
+      float x = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) x += s_o[k][tid];
+      p.out[w.s * p.os[0] + (w.hq0 + g) * p.os[1] + tid] = narrow<BF16>(x / ml.y);
+    }
+    if (tid == 0 && p.lse != nullptr)
+      p.lse[static_cast<int64_t>(w.s) * p.Hq + w.hq0 + g] = (ml.x + log2f(ml.y)) * 0.6931471805599453f;
+    __syncthreads();
+  }
+  if (p.weights == nullptr) return;
+  // ---- weights of the tokens of this CTA's share of the granules (units that one CTA finished have theirs, unless a
+  // kv head has several units: their shares of a token's weight are added here, in the order of the heads)
+  const int gs = p.gran_shift;
+  int at = static_cast<int>(static_cast<int64_t>(total) * blockIdx.x / gridDim.x);
+  const int stop = static_cast<int>(static_cast<int64_t>(total) * (blockIdx.x + 1) / gridDim.x);
+  if (at >= stop) return;
+  int lo = 0, hi = p.units;                           // the last unit that begins at or before `at`
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.ws_prefix[mid] <= at) lo = mid;
+    else hi = mid;
+  }
+  constexpr int kPerThread = 4;
+  for (int u = lo; at < stop; ++u) {
+    const int a = p.ws_prefix[u], b = p.ws_prefix[u + 1];
+    if (a == b) continue;
+    const int from = at - a;
+    at = min(b, stop);
+    if (u % p.chunks != 0 || (p.chunks == 1 && pieces_of(a, b, share).n == 1)) continue;
+    const UnitHeads w = unit_heads(p, u);
+    const int n = min(paged_count(p.v, p.lens[u / p.chunks]), (at - a) << gs);
+    for (int t0 = from << gs; t0 < n; t0 += kJoinThreads * kPerThread) {
+      float add[kPerThread] = {};
+      for (int c = 0; c < p.chunks; ++c) {
+        const int ca = p.ws_prefix[u + c];
+        const Pieces r = pieces_of(ca, ca + (b - a), share);
+        const int nh = unit_heads(p, u + c).n;
+        __syncthreads();
+        for (int g = warp; g < nh; g += kWarps) {
+          float lse;
+          if (r.n == 1) {
+            lse = p.ws_lse[static_cast<int64_t>(u + c) * GP + g];
+          } else {
+            const float2 ml = join_ml<GP>(p, r, g, lane);
+            lse = ml.x + log2f(ml.y);
+          }
+          if (lane == 0) s_lse[g] = lse;
+        }
+        __syncthreads();
+        const float* xs = p.ws_x + static_cast<int64_t>(u + c) * GP * p.x_stride;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+          const int t = t0 + i * kJoinThreads + tid;
+          if (t < n)
+            for (int g = 0; g < nh; ++g) add[i] += exp2_fast(xs[g * p.x_stride + t] - s_lse[g]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kPerThread; ++i) {
+        const int t = t0 + i * kJoinThreads + tid;
+        if (t >= n) continue;
+        const int pg = paged_page(p.v, w.s, t >> p.v.page_shift);
+        if (pg >= 0)
+          atomicAdd(p.weights + (static_cast<int64_t>(pg) * p.v.Hkv + w.h) * p.v.page + (t & (p.v.page - 1)), add[i]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host
+struct PagedPlan {
+  int chunks, gp, units, gran_shift, grid, whole, min_share;
+  int64_t cap;
+  size_t off_ml, off_o, off_lse, off_x, bytes;
+};
+
+static int paged_plan(const we_b200_paged_geom& g, int Hq, bool accumulate, PagedPlan* r) {
+  const int group = Hq / g.Hkv;
+  r->chunks = (group + kMaxGroup - 1) / kMaxGroup;
+  const int n = group < kMaxGroup ? group : kMaxGroup;
+  r->gp = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : n <= 8 ? 8 : 16;
+  const int64_t units = static_cast<int64_t>(g.S) * g.Hkv * r->chunks;
+  r->gran_shift = g.page == 16 ? 4 : 5;
+  r->cap = static_cast<int64_t>(g.max_pages) * g.page;
+  const int64_t most = units * (r->cap >> r->gran_shift);           // granules, counted in 32 bits by the kernels
+  if (units > (1 << 24) || most > 0x3FFFFFFF) return WE_B200_E_LIMIT;
+  r->units = static_cast<int>(units);
+  r->min_share = kTile >> r->gran_shift;                            // no less than a tile per CTA
+  r->whole = r->cap <= kWholeUnitTokens || r->units == 0;
+  const int64_t want = r->whole ? units : (most + r->min_share - 1) / r->min_share;
+  const int sms = sm_count();
+  r->grid = static_cast<int>(want < sms ? want : sms);
+  auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
+  if (r->whole) {
+    r->off_ml = r->off_o = r->off_lse = 0;
+    r->off_x = up(sizeof(float) * r->units * r->gp);
+  } else {
+    r->off_ml = up(sizeof(int32_t) * (r->units + 1));
+    r->off_o = r->off_ml + up(sizeof(float2) * 2 * r->grid * r->gp);
+    r->off_lse = r->off_o + sizeof(float) * 2 * r->grid * r->gp * g.Dh;
+    r->off_x = r->off_lse + up(sizeof(float) * r->units * r->gp);
+  }
+  r->bytes = accumulate ? r->off_x + sizeof(float) * static_cast<size_t>(r->units) * r->gp * r->cap
+                        : (r->whole ? 0 : r->off_x);
+  return WE_B200_OK;
+}
+
+// One map for both planes: (64 columns, 8 rows, column chunks, groups of 8 rows, pages and heads).  The last axis steps
+// by the greatest common divisor of the plane, page and head strides, so any of them can lie anywhere.
+static int paged_map(CUtensorMap* m, const void* kv, const we_b200_paged_geom& g, int gran, PagedAttnParams* p) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return WE_B200_E_DRIVER;
+  auto gcd = [](int64_t a, int64_t b) {
+    while (b != 0) {
+      const int64_t t = a % b;
+      a = b;
+      b = t;
+    }
+    return a;
+  };
+  const int64_t page_s = g.n_pages > 1 ? g.page_stride : 0, head_s = g.Hkv > 1 ? g.head_stride : 0;
+  int64_t step = gcd(gcd(g.plane_stride, page_s), head_s);
+  if (step == 0) step = g.token_stride;
+  p->unit_plane = g.plane_stride / step;
+  p->unit_page = page_s / step;
+  p->unit_head = head_s / step;
+  const int64_t top = p->unit_plane + (g.n_pages - 1) * p->unit_page + (g.Hkv - 1) * p->unit_head;
+  if (top >= 0x7FFFFFFF || step * 2 >= (1ll << 40) || g.token_stride * 16 >= (1ll << 40)) return WE_B200_E_LIMIT;
+  const cuuint32_t chunks = static_cast<cuuint32_t>(g.Dh / 64);
+  const cuuint64_t dims[5] = {64, 8, chunks, static_cast<cuuint64_t>(g.page / 8), static_cast<cuuint64_t>(top + 1)};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(g.token_stride * 2), 128,
+                                 static_cast<cuuint64_t>(g.token_stride * 16), static_cast<cuuint64_t>(step * 2)};
+  const cuuint32_t box[5] = {64, 8, chunks, static_cast<cuuint32_t>(gran / 8), 1};
+  const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+  const CUtensorMapDataType dt =
+      g.dtype == WE_B200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUresult rc = fn(m, dt, 5, const_cast<void*>(kv), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? WE_B200_OK : WE_B200_E_DRIVER;
+}
+
+template <int DH, bool BF16, int GP>
+static int launch_paged(const CUtensorMap& tm, const PagedAttnParams& p, cudaStream_t stream) {
+  using C = PagedCfg<DH, GP>;
+  static std::atomic<bool> done[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 0 || dev >= kMaxDevices) return WE_B200_E_LIMIT;
+  if (!done[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(paged_attn_kernel<DH, BF16, GP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return static_cast<int>(e);
+    }
+    done[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.grid), 1, 1);
+  cfg.blockDim = dim3(kPagedThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<DH, BF16, GP>, tm, p);
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  if (e == cudaSuccess && !p.whole) {
+    // as many CTAs as there can be heads to join or blocks of tokens to give their weights to
+    const int64_t items = static_cast<int64_t>(p.units) * (p.group < kMaxGroup ? p.group : kMaxGroup);
+    const int64_t most = p.weights != nullptr ? 4 * sm_count() : items;
+    cfg.gridDim = dim3(static_cast<unsigned>(most < 4 * sm_count() ? most : 4 * sm_count()), 1, 1);
+    cfg.blockDim = dim3(kJoinThreads, 1, 1);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<DH, BF16, GP>, p);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+  }
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const cudaError_t e2 = cudaGetLastError();
+  return e2 == cudaSuccess ? WE_B200_OK : static_cast<int>(e2);
+}
+
+template <int DH, bool BF16>
+static int launch_group(int gp, const CUtensorMap& tm, const PagedAttnParams& p, cudaStream_t stream) {
+  switch (gp) {
+    case 1: return launch_paged<DH, BF16, 1>(tm, p, stream);
+    case 2: return launch_paged<DH, BF16, 2>(tm, p, stream);
+    case 4: return launch_paged<DH, BF16, 4>(tm, p, stream);
+    case 8: return launch_paged<DH, BF16, 8>(tm, p, stream);
+    default: return launch_paged<DH, BF16, 16>(tm, p, stream);
+  }
 }
 
 }  // namespace we
 
 extern "C" size_t we_b200_paged_attn_workspace_bytes(const we_b200_paged_geom* g, int32_t Hq, int accumulate) {
-  (void)g;
-  (void)Hq;
-  (void)accumulate;
-  return 0;
+  we::PagedPlan plan;
+  if (g == nullptr || we::check_paged_geom(*g) != WE_B200_OK || Hq < 1 || Hq % g->Hkv != 0) return 0;
+  return we::paged_plan(*g, Hq, accumulate != 0, &plan) == WE_B200_OK ? plan.bytes : 0;
 }
 
 extern "C" int we_b200_paged_attn(const we_b200_paged_attn_args* a, int32_t* status, void* stream) {
   using namespace we;
   if (a == nullptr) return WE_B200_E_NULL;
   const we_b200_paged_geom& g = a->geom;
-  const int rc = check_paged_geom(g);
+  int rc = check_paged_geom(g);
   if (rc != WE_B200_OK) return rc;
   if (!a->q || !a->out || !a->kv || !a->table || !a->lens) return WE_B200_E_NULL;
   if (a->Hq < 1 || a->Hq % g.Hkv != 0) return WE_B200_E_SHAPE;
@@ -118,33 +880,38 @@ extern "C" int we_b200_paged_attn(const we_b200_paged_attn_args* a, int32_t* sta
     if ((a->q_strides[i] | a->out_strides[i]) & 7) return WE_B200_E_ALIGN;
   }
   if (!aligned16(a->q) || !aligned16(a->out) || !aligned16(a->kv)) return WE_B200_E_ALIGN;
+  PagedPlan plan;
+  if ((rc = paged_plan(g, a->Hq, a->weights != nullptr, &plan)) != WE_B200_OK) return rc;
+  if (plan.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < plan.bytes)) return WE_B200_E_WORKSPACE;
+  if (!aligned16(a->workspace)) return WE_B200_E_ALIGN;
   PagedAttnParams p;
   p.v = paged_view(g, a->table, status);
   p.q = static_cast<const uint16_t*>(a->q);
   p.out = static_cast<uint16_t*>(a->out);
   for (int i = 0; i < 2; ++i) p.qs[i] = a->q_strides[i], p.os[i] = a->out_strides[i];
-  p.kv = static_cast<const uint16_t*>(a->kv);
   p.lens = a->lens;
   p.weights = a->weights;
   p.lse = a->lse;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p.ws_prefix = reinterpret_cast<int32_t*>(ws);
+  p.ws_ml = reinterpret_cast<float2*>(ws + plan.off_ml);
+  p.ws_o = reinterpret_cast<float*>(ws + plan.off_o);
+  p.ws_lse = reinterpret_cast<float*>(ws + plan.off_lse);
+  p.ws_x = reinterpret_cast<float*>(ws + plan.off_x);
+  p.x_stride = plan.cap;
   p.Hq = a->Hq;
   p.group = a->Hq / g.Hkv;
+  p.chunks = plan.chunks;
+  p.units = plan.units;
+  p.grid = plan.grid;
+  p.gran_shift = plan.gran_shift;
+  p.whole = plan.whole;
+  p.min_share = plan.min_share;
   p.scale_log2 = (a->scale > 0.f ? a->scale : 1.0f / sqrtf(static_cast<float>(g.Dh))) * 1.4426950408889634f;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(g.Hkv), static_cast<unsigned>(g.S), 1);
-  cfg.blockDim = dim3(kPagedThreads, 1, 1);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e;
-  const bool bf16 = g.dtype == WE_B200_BF16;
-  if (g.Dh == 128) e = bf16 ? cudaLaunchKernelEx(&cfg, paged_attn_kernel<true, 128>, p) : cudaLaunchKernelEx(&cfg, paged_attn_kernel<false, 128>, p);
-  else e = bf16 ? cudaLaunchKernelEx(&cfg, paged_attn_kernel<true, 64>, p) : cudaLaunchKernelEx(&cfg, paged_attn_kernel<false, 64>, p);
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  const cudaError_t e2 = cudaGetLastError();
-  return e2 == cudaSuccess ? WE_B200_OK : static_cast<int>(e2);
+  CUtensorMap tm;
+  if ((rc = paged_map(&tm, a->kv, g, 1 << plan.gran_shift, &p)) != WE_B200_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (g.Dh == 128)
+    return g.dtype == WE_B200_BF16 ? launch_group<128, true>(plan.gp, tm, p, s) : launch_group<128, false>(plan.gp, tm, p, s);
+  return g.dtype == WE_B200_BF16 ? launch_group<64, true>(plan.gp, tm, p, s) : launch_group<64, false>(plan.gp, tm, p, s);
 }
