@@ -236,7 +236,8 @@ def test_append_under_a_budget(lens, T, keep, sink, recent, Dh, page, with_weigh
 
 @pytest.mark.parametrize("S,H,lens,T,keep,sink,recent", [
     (1, 2, [4096], 1, 4096, 4, 64), (2, 1, [5000, 4999], 300, 5000, 16, 1000), (1, 1, [20000], 1000, 20000, 0, 0),
-    (1, 1, [100], 9000, 777, 10, 100), (1, 2, [40000], 17, 33333, 4, 16)])
+    (1, 1, [100], 9000, 777, 10, 100), (1, 2, [40000], 17, 33333, 4, 16),
+    (1, 2, [40000], 3, 9000, 4, 16), (1, 1, [20000], 3, 40, 2, 8)])       # budgets lowered by much
 def test_long_budgets(S, H, lens, T, keep, sink, recent):
     c = Cache(S, H, 64, 64, -(-max(lens + [keep]) // 64), F16, seed=T, lens=lens)
     for step in range(2):

@@ -68,9 +68,24 @@ def test_bad_appends(lib, change, code):
 @pytest.mark.parametrize("change,code", [
     (dict(weights=None), -1), (dict(positions=None), -1), (dict(keep=0), -3), (dict(sink=-1), -3), (dict(recent=-1), -3),
     (dict(sink=90, recent=11), -3), (dict(sink=2 ** 31 - 1, recent=2 ** 31 - 1), -3), (dict(keep=321), -3),
-    (dict(workspace=None), -5), (dict(workspace_bytes=8), -5), (dict(workspace=FAKE + 1), -2)])
+    (dict(workspace=FAKE + 1), -2), (dict(weights=FAKE + 4), -2), (dict(positions=FAKE + 8), -2)])
 def test_bad_budgets(lib, change, code):
     assert lib.we_b200_paged_append_evict(ctypes.byref(append_args(**change)), None, None) == code
+
+
+def test_workspaces(lib):
+    # a table much wider than the budget: the lists of a session that holds that much need room
+    g = geom(max_pages=4096, table_stride=4096)
+    need = lib.we_b200_paged_evict_workspace_bytes(ctypes.byref(g), 8, 100)
+    assert need > 0
+    for change in (dict(workspace=None), dict(workspace_bytes=need - 1)):
+        assert lib.we_b200_paged_append_evict(ctypes.byref(append_args(g, **change)), None, None) == -5
+    need = lib.we_b200_paged_attn_workspace_bytes(ctypes.byref(g), 8, 0)
+    more = lib.we_b200_paged_attn_workspace_bytes(ctypes.byref(g), 8, 1)
+    assert 0 < need < more
+    for change in (dict(workspace=None), dict(workspace_bytes=need - 1), dict(weights=FAKE, workspace_bytes=more - 1)):
+        assert lib.we_b200_paged_attn(ctypes.byref(attn_args(g, **change)), None, None) == -5
+    assert lib.we_b200_paged_attn(ctypes.byref(attn_args(g, workspace=FAKE + 4)), None, None) == -2
 
 
 @pytest.mark.parametrize("change,code", [
