@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
@@ -103,6 +104,15 @@ class PagedAttnArgs(ctypes.Structure):
     ]
 
 
+# The same three laid out for struct.pack: a call fills its arguments in one go (a ctypes structure takes several
+# microseconds to fill field by field).
+_GEOM_FORMAT = "8i5q"
+PAGED_APPEND_PACK = struct.Struct("=" + _GEOM_FORMAT + "2Q6q10Q3q2Q4i")
+PAGED_ATTN_PACK = struct.Struct("=" + _GEOM_FORMAT + "2Q4q7Qif")
+assert PAGED_APPEND_PACK.size == ctypes.sizeof(PagedAppendArgs)
+assert PAGED_ATTN_PACK.size == ctypes.sizeof(PagedAttnArgs)
+
+
 class WeB200Error(RuntimeError):
     def __init__(self, code: int, where: str, msg: str):
         super().__init__(f"{where}: {msg} (code {code})")
@@ -177,11 +187,11 @@ def load() -> ctypes.CDLL:
     for name in ("we_b200_paged_append", "we_b200_paged_append_evict"):
         fn = getattr(lib, name)
         fn.restype = c_int
-        fn.argtypes = [POINTER(PagedAppendArgs), c_void_p, c_void_p]
+        fn.argtypes = [c_void_p, c_void_p, c_void_p]        # a PagedAppendArgs, or its bytes
     lib.we_b200_paged_evict_workspace_bytes.restype = c_size_t
     lib.we_b200_paged_evict_workspace_bytes.argtypes = [POINTER(PagedGeom), c_int32, c_int32]
     lib.we_b200_paged_attn.restype = c_int
-    lib.we_b200_paged_attn.argtypes = [POINTER(PagedAttnArgs), c_void_p, c_void_p]
+    lib.we_b200_paged_attn.argtypes = [c_void_p, c_void_p, c_void_p]     # a PagedAttnArgs, or its bytes
     lib.we_b200_paged_attn_workspace_bytes.restype = c_size_t
     lib.we_b200_paged_attn_workspace_bytes.argtypes = [POINTER(PagedGeom), c_int32, c_int]
 

@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import CacheGeom, PagedAppendArgs, PagedAttnArgs, PagedGeom, PrologueArgs, Strides3
+from ._lib import CacheGeom, PagedGeom, PrologueArgs, Strides3
 
 _DTYPE_CODE = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
 
@@ -262,75 +262,108 @@ def block_mask_tables(mask_written: torch.Tensor, tokens_per_frame: int
 
 
 # ---------------------------------------------------------------- paged cache
-@functools.lru_cache(maxsize=256)
-def _paged_geom(shape, stride, dtype, table_shape, table_stride) -> PagedGeom:
-    """Geometry of a page pool kv[2, P, Hkv, page, Dh] (any strides, head dim contiguous) with a table [S, M]."""
+# A decoding step makes these calls for every layer, so their cost on the host counts: all checks of shapes, types,
+# strides and devices are one look-up of the values they depend on, and the arguments are packed in one go.
+_status_ptrs = {}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _meta(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _refuse_grad(*tensors) -> None:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError("the paged cache operators have no backward pass; call them under torch.no_grad()")
+
+
+def _check_paged(kv, table, counts, per_slot, others) -> Tuple[int, ...]:
+    """What every paged entry point checks; the geometry's fields."""
+    for meta in (kv, table, *counts, *per_slot, *others):
+        if meta is None:
+            continue
+        if meta[3] < 0:
+            raise RuntimeError("world_engine_b200 runs on CUDA tensors only (sm_100a); there is no CPU path")
+        if meta[3] != kv[3]:
+            raise ValueError("all tensors of a paged cache call must be on the device of kv")
+    shape, stride, dtype, _ = kv
     if len(shape) != 5 or shape[0] != 2 or stride[4] != 1:
         raise ValueError("kv must be [2, pages, Hkv, page, Dh] with a contiguous last axis")
-    if len(table_shape) != 2 or table_stride[1] != 1:
-        raise ValueError("table must be [S, max_pages] with contiguous rows")
     _, P, Hkv, page, Dh = shape
-    S, M = table_shape
-    return PagedGeom(S, Hkv, Dh, page, P, M, dtype_code(dtype), 0, stride[0], stride[1], stride[2], stride[3],
-                     table_stride[0])
-
-
-def _paged_check(kv, table, int32s, per_slot, others) -> PagedGeom:
-    """The checks every paged entry point makes: devices, types and shapes of the cache's tensors."""
-    device = kv.device
-    for t in (kv, table, *int32s, *per_slot, *others):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("world_engine_b200 runs on CUDA tensors only (sm_100a); there is no CPU path")
-        if t.device != device:
-            raise ValueError("all tensors of a paged cache call must be on the device of kv")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("the paged cache operators have no backward pass; call them under torch.no_grad()")
-    g = _paged_geom(kv.shape, kv.stride(), kv.dtype, table.shape, table.stride())
-    if table.dtype != torch.int32:
-        raise ValueError("table must be int32")
-    for t in int32s:
-        if t is not None and (t.dtype != torch.int32 or t.shape != (g.S, g.Hkv) or not t.is_contiguous()):
+    if len(table[0]) != 2 or table[1][1] != 1 or table[2] != torch.int32:
+        raise ValueError("table must be int32 [S, max_pages] with contiguous rows")
+    S, M = table[0]
+    for meta in counts:
+        if meta is not None and (meta[2] != torch.int32 or meta[0] != (S, Hkv) or not _dense(meta)):
             raise ValueError("token counts and positions must be contiguous int32 [S, Hkv]")
-    for t, dtype in zip(per_slot, (torch.float32, torch.int32)):
-        if t is not None and (t.dtype != dtype or t.shape != (g.n_pages, g.Hkv, g.page) or not t.is_contiguous()):
+    for meta, want in zip(per_slot, (torch.float32, torch.int32)):
+        if meta is not None and (meta[2] != want or meta[0] != (P, Hkv, page) or not _dense(meta)):
             raise ValueError("weights (float32) and positions (int32) must be contiguous [pages, Hkv, page]")
-    return g
+    return (S, Hkv, Dh, page, P, M, dtype_code(dtype), 0, stride[0], stride[1], stride[2], stride[3], table[1][0])
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return t.data_ptr() if t is not None else None
+def _dense(meta) -> bool:
+    want = 1
+    for n, s in zip(reversed(meta[0]), reversed(meta[1])):
+        if n != 1 and s != want:
+            return False
+        want *= n
+    return True
 
 
-def _call_on(device: torch.device, fn, args, where: str) -> None:
+def _call_paged(fn, args: bytes, index: int, where: str) -> None:
     """One library call on the device of the tensors and its current stream."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(args), status_word(device).data_ptr(), _stream_ptr(device))
+    status = _status_ptrs.get(index)
+    if status is None:
+        status = _status_ptrs[index] = status_word(torch.device("cuda", index)).data_ptr()
+    if index == torch.cuda.current_device():
+        rc = fn(args, status, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(ctypes.byref(args), status_word(device).data_ptr(), _stream_ptr(device))
-    _lib.check(rc, where)
+        with torch.cuda.device(index):
+            rc = fn(args, status, _raw_stream(index))
+    if rc:
+        _lib.check(rc, where)
 
 
-def _append_args(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new, lens_out,
-                 next_pos_out) -> PagedAppendArgs:
+@functools.lru_cache(maxsize=1024)
+def _append_plan(kv, table, lens, next_pos, lens_out, next_pos_out, k_new, v_new, n_new, weights, positions, w_new,
+                 keep):
+    """Checks of an append; (geometry, strides of k_new and v_new, strides of w_new, T, workspace bytes)."""
+    geom = _check_paged(kv, table, (lens, next_pos, lens_out, next_pos_out), (weights, positions),
+                        (k_new, v_new, n_new, w_new))
+    S, Hkv, Dh = geom[:3]
+    shape = k_new[0]
+    if len(shape) != 4 or (shape[0], shape[1], shape[3]) != (S, Hkv, Dh) or v_new[0] != shape \
+            or k_new[2] != kv[2] or v_new[2] != kv[2] or k_new[1][3] != 1 or v_new[1][3] != 1:
+        raise ValueError("k_new and v_new must be [S, Hkv, T, Dh] of the cache's type with a contiguous last axis")
+    if n_new is not None and (n_new[2] != torch.int32 or n_new[0] != (S,) or not _dense(n_new)):
+        raise ValueError("n_new must be contiguous int32 [S]")
+    if w_new is not None and (w_new[2] != torch.float32 or w_new[0] != shape[:3]):
+        raise ValueError("w_new must be float32 [S, Hkv, T]")
+    need = 0
+    if keep > 0:
+        need = _lib.load().we_b200_paged_evict_workspace_bytes(ctypes.byref(PagedGeom(*geom)), shape[2], keep)
+    return geom, (*k_new[1][:3], *v_new[1][:3]), w_new[1] if w_new is not None else (0, 0, 0), shape[2], need
+
+
+def _append(fn, where, kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new, lens_out,
+            next_pos_out, keep, sink, recent) -> None:
     lens_out = lens if lens_out is None else lens_out
     next_pos_out = next_pos if next_pos_out is None else next_pos_out
-    g = _paged_check(kv, table, (lens, next_pos, lens_out, next_pos_out), (weights, positions), (k_new, v_new, n_new, w_new))
-    S, Hkv, T, Dh = k_new.shape
-    if (S, Hkv, Dh) != (g.S, g.Hkv, g.Dh) or v_new.shape != k_new.shape or k_new.dtype != kv.dtype \
-            or v_new.dtype != kv.dtype:
-        raise ValueError("k_new and v_new must be [S, Hkv, T, Dh] of the cache's type")
-    if n_new is not None and (n_new.dtype != torch.int32 or n_new.shape != (S,) or not n_new.is_contiguous()):
-        raise ValueError("n_new must be contiguous int32 [S]")
-    if w_new is not None and (w_new.dtype != torch.float32 or w_new.shape != (S, Hkv, T)):
-        raise ValueError("w_new must be float32 [S, Hkv, T]")
-    return PagedAppendArgs(
-        g, k_new.data_ptr(), v_new.data_ptr(), _strides3(k_new), _strides3(v_new), kv.data_ptr(), _ptr(weights),
-        _ptr(positions), table.data_ptr(), lens.data_ptr(), next_pos.data_ptr(), lens_out.data_ptr(),
-        next_pos_out.data_ptr(), _ptr(n_new), _ptr(w_new),
-        Strides3(*w_new.stride()) if w_new is not None else Strides3(), None, 0, T, 0, 0, 0)
+    if torch.is_grad_enabled():
+        _refuse_grad(kv, k_new, v_new, weights, w_new)
+    geom, strides, w_strides, T, need = _append_plan(
+        _meta(kv), _meta(table), _meta(lens), _meta(next_pos), _meta(lens_out), _meta(next_pos_out), _meta(k_new),
+        _meta(v_new), _meta(n_new), _meta(weights), _meta(positions), _meta(w_new), keep)
+    ws = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
+    _call_paged(fn, _lib.PAGED_APPEND_PACK.pack(
+        *geom, k_new.data_ptr(), v_new.data_ptr(), *strides, kv.data_ptr(),
+        0 if weights is None else weights.data_ptr(), 0 if positions is None else positions.data_ptr(),
+        table.data_ptr(), lens.data_ptr(), next_pos.data_ptr(), lens_out.data_ptr(), next_pos_out.data_ptr(),
+        0 if n_new is None else n_new.data_ptr(), 0 if w_new is None else w_new.data_ptr(), *w_strides,
+        0 if ws is None else ws.data_ptr(), need, T, keep, sink, recent), kv.get_device(), where)
 
 
 def paged_append_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, next_pos: torch.Tensor,
@@ -343,8 +376,8 @@ def paged_append_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, nex
     given.  `k_new` / `v_new` are `[S, Hkv, T, Dh]` views (any strides, head dim contiguous); of a padded batch only
     the first `n_new[s]` tokens count.  The counts are updated in place unless `lens_out` / `next_pos_out` are
     given.  Tokens for which a session has no room are dropped and reported by `check_status`."""
-    args = _append_args(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new, lens_out, next_pos_out)
-    _call_on(kv.device, _lib.load().we_b200_paged_append, args, "we_b200_paged_append")
+    _append(_lib.load().we_b200_paged_append, "we_b200_paged_append", kv, table, lens, next_pos, k_new, v_new, n_new,
+            weights, positions, w_new, lens_out, next_pos_out, 0, 0, 0)
 
 
 def paged_append_evict_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, next_pos: torch.Tensor,
@@ -358,14 +391,26 @@ def paged_append_evict_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tenso
     left, so the order of a session's tokens is not kept (`positions` tells which is which)."""
     if weights is None or positions is None:
         raise ValueError("eviction needs weights and positions")
-    args = _append_args(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new, lens_out, next_pos_out)
-    args.keep, args.sink, args.recent = int(keep), int(sink), int(recent)
-    lib = _lib.load()
-    need = lib.we_b200_paged_evict_workspace_bytes(ctypes.byref(args.geom), args.T, args.keep)
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=kv.device)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _call_on(kv.device, lib.we_b200_paged_append_evict, args, "we_b200_paged_append_evict")
+    if not (0 < keep < 2 ** 31 and 0 <= sink and 0 <= recent and sink + recent <= keep):
+        raise ValueError("a budget needs 0 <= sink + recent <= keep and at least one token")
+    _append(_lib.load().we_b200_paged_append_evict, "we_b200_paged_append_evict", kv, table, lens, next_pos, k_new,
+            v_new, n_new, weights, positions, w_new, lens_out, next_pos_out, keep, sink, recent)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attn_plan(q, kv, table, lens, weights, out, lse):
+    """Checks of an attention call; (geometry, workspace bytes)."""
+    geom = _check_paged(kv, table, (lens,), (weights,), (q, out, lse))
+    S, _, Dh = geom[:3]
+    shape = q[0]
+    if len(shape) != 4 or (shape[0], shape[2], shape[3]) != (S, 1, Dh) or q[2] != kv[2] or q[1][3] != 1:
+        raise ValueError("q must be [S, Hq, 1, Dh] of the cache's type with a contiguous last axis")
+    if out is not None and (out[0] != shape or out[2] != q[2] or out[1][3] != 1):
+        raise ValueError("out must have q's shape and type and a contiguous last axis")
+    if lse is not None and (lse[2] != torch.float32 or lse[0] != shape[:2] or not _dense(lse)):
+        raise ValueError("lse must be contiguous float32 [S, Hq]")
+    need = _lib.load().we_b200_paged_attn_workspace_bytes(ctypes.byref(PagedGeom(*geom)), shape[1], weights is not None)
+    return geom, need
 
 
 def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float = 0.0,
@@ -375,23 +420,18 @@ def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: tor
     `[S, Hq, 1, Dh]` view; the output has its shape.  With `weights` the softmax weight every held token is given
     (summed over the query heads of its kv head) is added to it in place; `lse` (float32 `[S, Hq]`, contiguous)
     receives the logarithm of the softmax sum.  A kv head that holds nothing gives 0 and -inf."""
-    g = _paged_check(kv, table, (lens,), (weights,), (q, out, lse))
-    S, Hq, T, Dh = q.shape
-    if (S, T, Dh) != (g.S, 1, g.Dh) or q.dtype != kv.dtype or q.stride(3) != 1:
-        raise ValueError("q must be [S, Hq, 1, Dh] of the cache's type with a contiguous last axis")
+    if torch.is_grad_enabled():
+        _refuse_grad(q, kv, weights, out, lse)
+    geom, need = _attn_plan(_meta(q), _meta(kv), _meta(table), _meta(lens), _meta(weights), _meta(out), _meta(lse))
+    Hq = q.shape[1]
     if out is None:
-        out = torch.empty((S, Hq, 1, Dh), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
-        raise ValueError("out must have q's shape and type and a contiguous last axis")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (S, Hq) or not lse.is_contiguous()):
-        raise ValueError("lse must be contiguous float32 [S, Hq]")
-    lib = _lib.load()
-    need = lib.we_b200_paged_attn_workspace_bytes(ctypes.byref(g), Hq, weights is not None)
+        out = q.new_empty((geom[0], Hq, 1, geom[2]))
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     qs, os_ = q.stride(), out.stride()
-    args = PagedAttnArgs(g, q.data_ptr(), out.data_ptr(), (qs[0], qs[1]), (os_[0], os_[1]), kv.data_ptr(),
-                         table.data_ptr(), lens.data_ptr(), _ptr(weights), _ptr(lse), _ptr(ws), need, Hq, scale)
-    _call_on(q.device, lib.we_b200_paged_attn, args, "we_b200_paged_attn")
+    _call_paged(_lib.load().we_b200_paged_attn, _lib.PAGED_ATTN_PACK.pack(
+        *geom, q.data_ptr(), out.data_ptr(), qs[0], qs[1], os_[0], os_[1], kv.data_ptr(), table.data_ptr(),
+        lens.data_ptr(), 0 if weights is None else weights.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        0 if ws is None else ws.data_ptr(), need, Hq, scale), q.get_device(), "we_b200_paged_attn")
     return out
 
 
