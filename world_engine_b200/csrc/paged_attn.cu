@@ -13,16 +13,19 @@
 // lies in one CTA is finished there; of one that several CTAs share each leaves (m, l, O) in the workspace and
 // paged_join_kernel puts them together, in the order of the tokens.
 //
-// One CTA per SM, 256 threads:
-//   warps 0-3  softmax.  Thread t owns token t of a tile (TMEM lane t): its logits of the G heads are G columns.  The
-//              reference m_g is raised only when a logit exceeds it by more than 8 (then O is rescaled in tensor
-//              memory), so a tile costs one vote among the 128 threads and no reduction.  P goes to shared memory as
-//              the sum of two 16-bit numbers in two columns: the second column costs nothing (N is at least 16) and
-//              leaves the weights accurate to 2^-16 instead of 2^-8.
-//   warp 4     K: walks the run, publishes the segments with their Q rows, loads the K tiles
-//   warp 7     V tiles (a ring of its own)
-//   warp 5     issues S^T, warp 6 issues O^T (one thread each)
-// Tensor memory (64 columns): S0, S1 (16 each), O (high and low parts of up to 16 heads: 32).
+// One CTA per SM, 384 threads:
+//   warps 0-7  softmax, two groups of 128 threads that take tiles in turn, each with statistics and an accumulator of
+//              its own (put together at the end of a segment).  Thread t of a group owns token t of a tile (TMEM
+//              lane t): its logits of the G heads are G columns.  The reference m_g is raised only when a logit
+//              exceeds it by more than 8 (then O is rescaled in tensor memory), so a tile costs one vote among the
+//              128 threads and no reduction.  P goes to shared memory as the sum of two 16-bit numbers in two
+//              columns: the second column costs nothing (N is at least 16) and leaves the weights accurate to 2^-16
+//              instead of 2^-8.  A token's columns lie next to each other (P is an MN-major operand): one or two
+//              16-byte stores per token.
+//   warp 8     K: walks the run, publishes the segments with their Q rows, loads the K tiles
+//   warp 11    V tiles (a ring of its own)
+//   warp 9     issues S^T, warp 10 issues O^T (one thread each)
+// Tensor memory (128 columns): four S buffers of 16, O of either group (high and low parts of up to 16 heads: 32).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -32,9 +35,14 @@
 
 namespace we {
 
-constexpr int kPagedThreads = 256;
+constexpr int kPagedThreads = 384;
+constexpr int kPagedWarps = kPagedThreads / 32;
 constexpr int kTile = 128;                 // tokens per tile
 constexpr int kSegs = 4;                   // segments in flight
+constexpr int kBufs = 4;                   // S buffers
+constexpr uint32_t kTmemColumns = 128;
+constexpr uint32_t kColO = 64;             // + 32 per group
+constexpr float kFloor = -1.0e38f;         // the reference before the first logit
 constexpr int kMaxGroup = 16;              // query heads per unit
 constexpr float kRaise = 8.0f;             // log2 units by which a logit may exceed the reference
 constexpr int kJoinThreads = 256;
@@ -79,6 +87,16 @@ __device__ __forceinline__ float widen(uint16_t x) {
   if constexpr (BF16) return __uint_as_float(static_cast<uint32_t>(x) << 16);
   else return __half2float(__ushort_as_half(x));
 }
+template <bool BF16>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {           // a in the low half
+  if constexpr (BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -108,13 +126,17 @@ struct PagedCfg {
   static constexpr int kStages = DH == 128 ? 3 : 6;
   static constexpr int kNP = 2 * GP <= 16 ? 16 : 32;         // columns of O^T
   static constexpr int kQBytes = 16 * DH * 2;                // [chunk][16 rows][128 bytes]
-  static constexpr int kPBytes = 2 * kNP * 128;              // [64 tokens][kNP rows][128 bytes]
+  static constexpr int kPRow = 2 * kNP;                      // a token's columns: 32 or 64 bytes, swizzled as such
+  static constexpr int kPBytes = kTile * kPRow;
+  static_assert(GP * 128 * 4 <= kPBytes, "a group's O passes through its P buffer");
   static constexpr int kOffV = kStages * kTileBytes;
   static constexpr int kOffQ = 2 * kStages * kTileBytes;
   static constexpr int kOffP = kOffQ + kSegs * kQBytes;
   static constexpr int kOffAux = kOffP + 2 * kPBytes;
-  static constexpr int kAux = 512 + 2 * 4 * 16 * 4 + 64 + 64;
+  static constexpr int kAux = 384 + 2 * 512 + 192 + kSegs * 16 + 128;
+  static_assert((4 * kStages + 2 * kSegs + 2 * kBufs + 2) * 8 <= 384, "barriers");
   static constexpr int kSmem = kOffAux + kAux + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 // The heads of a unit.
@@ -163,18 +185,19 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   uint64_t* q_full = v_empty + C::kStages;
   uint64_t* q_empty = q_full + kSegs;
   uint64_t* s_full = q_empty + kSegs;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* pv_done = p_full + 2;
-  float* s_max = reinterpret_cast<float*>(aux + 512);                 // [4 warps][16]
-  float* s_sum = s_max + 64;                                          // [4 warps][16]
-  Segment* segs = reinterpret_cast<Segment*>(aux + 1024);
-  int* s_plan = reinterpret_cast<int*>(aux + 1024 + kSegs * 16);      // 0 unit, 1 granule, 2 run, 4.. scan
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_plan + 14);
-  volatile int* s_abort = s_plan + 15;
+  uint64_t* p_full = s_full + kBufs;
+  uint64_t* pv_done = p_full + kBufs;
+  float* s_max = reinterpret_cast<float*>(aux + 384);                 // [2 groups][4 warps][16]
+  float* s_sum = s_max + 128;                                         // [2 groups][4 warps][16]
+  float* s_join = s_sum + 128;                                        // group 1's m and l, lse: [3][16]
+  Segment* segs = reinterpret_cast<Segment*>(aux + 1600);
+  int* s_plan = reinterpret_cast<int*>(aux + 1600 + kSegs * 16);      // 0 unit, 1 granule, 2 run, 4.. scan
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_plan + 30);
+  volatile int* s_abort = s_plan + 31;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
-  if (warp == 5) {
-    tmem_alloc(s_tmem, 64);
+  if (warp == 9) {
+    tmem_alloc(s_tmem, kTmemColumns);
     tmem_relinquish();
   }
   if (tid == 0) {
@@ -186,13 +209,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     }
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 7);         // four softmax warps, both issuers, the V producer
+      mbar_init(&q_empty[i], 11);        // eight softmax warps, both issuers, the V producer
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kBufs; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
-      mbar_init(&pv_done[i], 1);
     }
+    mbar_init(&pv_done[0], 1);
+    mbar_init(&pv_done[1], 1);
     *s_abort = 0;
     fence_mbar_init();
   }
@@ -231,7 +255,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     if (lane == 31) s_plan[4 + warp] = pre;
     __syncthreads();
     int total = 0;
-    for (int w = 0; w < kPagedThreads / 32; ++w) {
+    for (int w = 0; w < kPagedWarps; ++w) {
       const int y = s_plan[4 + w];
       if (w < warp) pre += y;
       total += y;
@@ -261,9 +285,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   tc_fence_after();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = *s_tmem;
-  constexpr uint32_t kColO = 32;
-
-  if (warp == 4) {
+  if (warp == 8) {
     // ---------------------------------------------------------------- K tiles and segments
     int u = s_plan[0], at = s_plan[1], left = s_plan[2];
     int seg = 0, it = 0;
@@ -339,7 +361,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
       segs[seg % kSegs].ntok = 0;
       mbar_arrive(&q_full[seg % kSegs]);
     }
-  } else if (warp == 7) {
+  } else if (warp == 11) {
     // ---------------------------------------------------------------- V tiles
     int it = 0;
     for (int seg = 0;; ++seg) {
@@ -372,7 +394,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
         pg = pg_next;
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // ---------------------------------------------------------------- S^T = K Q^T: 128 tokens x 16 heads
     if (lane == 0) {
       constexpr uint32_t kIdesc = umma_idesc(BF16 ? 1u : 0u, 0u, kTile, 16);
@@ -388,25 +410,25 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
         for (int t0 = 0; t0 < ntok && ok; t0 += kTile, ++it) {
           const int st = it % C::kStages;
           ok = mbar_wait(&k_full[st], (it / C::kStages) & 1, s_abort);
-          if (it >= 2) ok = mbar_wait(&p_full[it & 1], ((it - 2) >> 1) & 1, s_abort) && ok;    // S(it - 2) was read
+          if (it >= kBufs) ok = mbar_wait(&p_full[it % kBufs], ((it / kBufs) - 1) & 1, s_abort) && ok;   // the buffer was read
           if (!ok) break;
           tc_fence_after();
           const uint32_t k_lo = umma_desc_lo(smem_u32(sK + st * C::kTileBytes), 16);
 #pragma unroll
           for (int kk = 0; kk < DH / 16; ++kk)
-            umma_ss(tmem + 16 * (it & 1), k_lo + (kk >> 2) * 64 + (kk & 3) * 2, kHiK, q_lo + (kk >> 2) * 128 + (kk & 3) * 2,
+            umma_ss(tmem + 16 * (it % kBufs), k_lo + (kk >> 2) * 64 + (kk & 3) * 2, kHiK, q_lo + (kk >> 2) * 128 + (kk & 3) * 2,
                     kHiQ, kIdesc, kk > 0);
-          tc_commit(&s_full[it & 1]);
+          tc_commit(&s_full[it % kBufs]);
           tc_commit(&k_empty[st]);
         }
         tc_commit(&q_empty[qslot]);
       }
     }
-  } else if (warp == 6) {
+  } else if (warp == 10) {
     // ---------------------------------------------------------------- O^T += V^T P^T: 128 rows (of the head dim) x heads
     if (lane == 0) {
-      constexpr uint32_t kIdesc = umma_idesc(BF16 ? 1u : 0u, 0u, 128, C::kNP) | (1u << 15);     // A is MN-major
-      constexpr uint32_t kHiV = umma_desc_hi(C::kRowGroup), kHiP = umma_desc_hi(1024);
+      constexpr uint32_t kIdesc = umma_idesc(BF16 ? 1u : 0u, 1u, 128, C::kNP) | (1u << 15);     // both MN-major
+      constexpr uint32_t kHiV = umma_desc_hi(C::kRowGroup), kHiP = umma_desc_hi(8 * C::kPRow, C::kPRow == 32 ? 6 : 4);
       int it = 0;
       bool ok = true;
       for (int seg = 0; ok; ++seg) {
@@ -418,7 +440,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
         for (int t0 = 0; t0 < ntok && ok; t0 += kTile, ++it) {
           const int st = it % C::kStages, steps = (min(kTile, ntok - t0) + 15) >> 4;
           ok = mbar_wait(&v_full[st], (it / C::kStages) & 1, s_abort);
-          ok = mbar_wait(&p_full[it & 1], (it >> 1) & 1, s_abort) && ok;
+          ok = mbar_wait(&p_full[it % kBufs], (it / kBufs) & 1, s_abort) && ok;
           if (!ok) break;
           tc_fence_after();
           // (head dim 64: rows 64.. of the product read the next eight tokens in place of a second column chunk;
@@ -426,8 +448,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
           const uint32_t v_lo = umma_desc_lo(smem_u32(sV + st * C::kTileBytes), 1024);
           const uint32_t p_lo = umma_desc_lo(smem_u32(sP + (it & 1) * C::kPBytes), 16);
           for (int kk = 0; kk < steps; ++kk)
-            umma_ss(tmem + kColO, v_lo + kk * (2 * C::kRowGroup >> 4), kHiV, p_lo + (kk >> 2) * (C::kNP * 128 >> 4) + (kk & 3) * 2,
-                    kHiP, kIdesc, t0 > 0 || kk > 0);
+            umma_ss(tmem + kColO + 32 * (it & 1), v_lo + kk * (2 * C::kRowGroup >> 4), kHiV, p_lo + kk * C::kPRow, kHiP,
+                    kIdesc, t0 >= 2 * kTile || kk > 0);
           tc_commit(&v_empty[st]);
           tc_commit(&pv_done[it & 1]);
         }
@@ -435,152 +457,215 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    const int grp = warp >> 2, row = tid & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t o_col = tmem + lanes + kColO + 32 * grp;
+    float* my_max = s_max + 64 * grp;
+    float* my_sum = s_sum + 64 * grp;
+    float* other_o = reinterpret_cast<float*>(sP + C::kPBytes);         // [GP][128], in group 1's P buffer
+    uint8_t* p_row = sP + grp * C::kPBytes + row * C::kPRow;
+    const uint32_t swz = C::kPRow == 32 ? (row >> 2) & 1 : (row >> 1) & 3;
     int it = 0;
     for (int seg = 0;; ++seg) {
       const int qslot = seg % kSegs;
       const bool ok = mbar_wait(&q_full[qslot], (seg / kSegs) & 1, s_abort);
       __syncwarp();
-      if (bar_any(1, 128, !ok)) break;
+      if (bar_any(1, 256, !ok)) break;
       const Segment d = segs[qslot];
       if (d.ntok == 0) break;
       const UnitHeads w = unit_heads(p, d.unit);
       float m[GP], l[GP];
 #pragma unroll
-      for (int g = 0; g < GP; ++g) m[g] = -INFINITY, l[g] = 0.f;
+      for (int g = 0; g < GP; ++g) m[g] = kFloor, l[g] = 0.f;
       float* xs = p.weights != nullptr ? p.ws_x + static_cast<int64_t>(d.unit) * GP * p.x_stride + d.tok0 : nullptr;
+      int last = -1;                                       // this group's last tile
       for (int t0 = 0; t0 < d.ntok; t0 += kTile, ++it) {
-        const int buf = it & 1, nv = min(kTile, d.ntok - t0);
-        mbar_wait(&s_full[buf], (it >> 1) & 1, s_abort);
+        if ((it & 1) != grp) continue;
+        const int nv = min(kTile, d.ntok - t0);
+        mbar_wait(&s_full[it % kBufs], (it / kBufs) & 1, s_abort);
         __syncwarp();
         tc_fence_after();
         uint32_t raw[GP];
-        tmem_ld_n<GP>(tmem + lanes + 16 * buf, raw);
+        tmem_ld_n<GP>(tmem + lanes + 16 * (it % kBufs), raw);
         tmem_ld_wait();
-        float x[GP];
-        bool raise = false;
+        float x[GP], e[GP];
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          x[g] = tid < nv && g < w.n ? __uint_as_float(raw[g]) * p.scale_log2 : -INFINITY;
-          raise |= x[g] > m[g] + kRaise;
+        for (int g = 0; g < GP; ++g) x[g] = __uint_as_float(raw[g]) * p.scale_log2;
+        if (w.n < GP) {
+#pragma unroll
+          for (int g = 1; g < GP; ++g)
+            if (g >= w.n) x[g] = -INFINITY;
         }
-        if (xs != nullptr && tid < nv) {
+        if (row >= nv) {
+#pragma unroll
+          for (int g = 0; g < GP; ++g) x[g] = -INFINITY;
+        } else if (xs != nullptr) {
 #pragma unroll
           for (int g = 0; g < GP; ++g)
-            if (g < w.n) xs[g * p.x_stride + t0 + tid] = x[g];
+            if (g < w.n) xs[g * p.x_stride + t0 + row] = x[g];
         }
-        if (bar_any(1, 128, raise)) {
+        float over = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          e[g] = x[g] - m[g];
+          over = fmaxf(over, e[g]);
+        }
+        if (bar_any(2 + grp, 128, over > kRaise)) {
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
             float t = x[g];
             for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-            if (lane == 0) s_max[warp * 16 + g] = t;
+            if (lane == 0) my_max[(warp & 3) * 16 + g] = t;
           }
-          bar_sync(1, 128);
+          bar_sync(2 + grp, 128);
           float f[GP];
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
-            const float t = fmaxf(fmaxf(fmaxf(s_max[g], s_max[16 + g]), fmaxf(s_max[32 + g], s_max[48 + g])), m[g]);
+            const float t = fmaxf(fmaxf(fmaxf(my_max[g], my_max[16 + g]), fmaxf(my_max[32 + g], my_max[48 + g])), m[g]);
             f[g] = t == m[g] ? 1.f : exp2_fast(m[g] - t);
             m[g] = t;
             l[g] *= f[g];
+            e[g] = x[g] - t;
           }
-          if (t0 > 0) {
-            mbar_wait(&pv_done[buf ^ 1], ((it - 1) >> 1) & 1, s_abort);
+          if (last >= 0) {
+            mbar_wait(&pv_done[grp], (last >> 1) & 1, s_abort);
             __syncwarp();
             tc_fence_after();
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
               uint32_t o[GP];
-              tmem_ld_n<GP>(tmem + lanes + kColO + part * GP, o);
+              tmem_ld_n<GP>(o_col + part * GP, o);
               tmem_ld_wait();
 #pragma unroll
               for (int g = 0; g < GP; ++g) o[g] = __float_as_uint(__uint_as_float(o[g]) * f[g]);
-              tmem_st_n<GP>(tmem + lanes + kColO + part * GP, o);
+              tmem_st_n<GP>(o_col + part * GP, o);
             }
             tmem_st_wait();
           }
         }
-        if (it >= 2) mbar_wait(&pv_done[buf], ((it - 2) >> 1) & 1, s_abort);      // P(it - 2) was read
-        uint8_t* pw = sP + buf * C::kPBytes + (tid >> 6) * (C::kNP * 128);
-        const uint32_t col = (tid & 63) * 2;
+        uint32_t words[GP == 1 ? 1 : GP];                  // GP high parts, then GP low parts
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
-          const float e = exp2_fast(x[g] - (m[g] == -INFINITY ? 0.f : m[g]));
-          l[g] += e;
-          const uint16_t hi = narrow<BF16>(e);
-          const uint16_t lo = narrow<BF16>(e - widen<BF16>(hi));
-          *reinterpret_cast<uint16_t*>(pw + g * 128 + (col ^ ((g & 7) << 4))) = hi;
-          *reinterpret_cast<uint16_t*>(pw + (GP + g) * 128 + (col ^ (((GP + g) & 7) << 4))) = lo;
+          e[g] = exp2_fast(e[g]);
+          l[g] += e[g];
         }
-        if (tid >= nv && tid < ((nv + 15) & ~15)) {
+        if constexpr (GP == 1) {
+          const uint16_t hi = narrow<BF16>(e[0]);
+          words[0] = hi | (static_cast<uint32_t>(narrow<BF16>(e[0] - widen<BF16>(hi))) << 16);
+        } else {
+#pragma unroll
+          for (int g = 0; g < GP; g += 2) {
+            const uint32_t hi = narrow2<BF16>(e[g], e[g + 1]);
+            words[g / 2] = hi;
+            words[(GP + g) / 2] = narrow2<BF16>(e[g] - widen<BF16>(static_cast<uint16_t>(hi)),
+                                                e[g + 1] - widen<BF16>(static_cast<uint16_t>(hi >> 16)));
+          }
+        }
+        if (it >= 2) mbar_wait(&pv_done[grp], ((it - 2) >> 1) & 1, s_abort);      // the P before was read
+        if constexpr (GP == 1) {
+          *reinterpret_cast<uint32_t*>(p_row + (swz << 4)) = words[0];
+        } else if constexpr (GP == 2) {
+          *reinterpret_cast<uint2*>(p_row + (swz << 4)) = make_uint2(words[0], words[1]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < GP / 4; ++c)
+            *reinterpret_cast<uint4*>(p_row + ((c ^ swz) << 4)) =
+                make_uint4(words[4 * c], words[4 * c + 1], words[4 * c + 2], words[4 * c + 3]);
+        }
+        if (row >= nv && row < ((nv + 15) & ~15)) {
           // rows behind the last token: whatever the page holds there must not meet a weight of zero
           const int st = it % C::kStages;
           mbar_wait(&v_full[st], (it / C::kStages) & 1, s_abort);
-          uint8_t* row = sV + st * C::kTileBytes + (tid >> 3) * C::kRowGroup + (tid & 7) * 128;
+          uint8_t* v_row = sV + st * C::kTileBytes + (row >> 3) * C::kRowGroup + (row & 7) * 128;
 #pragma unroll
           for (int c = 0; c < C::kChunks; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(row + c * 1024 + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(v_row + c * 1024 + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
         }
         __syncwarp();
         fence_proxy_async_smem();
         tc_fence_before();
-        mbar_arrive(&p_full[buf]);
+        mbar_arrive(&p_full[it % kBufs]);
+        last = it;
       }
-      // ---- the segment's sums
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        for (int o = 16; o > 0; o >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
-        if (lane == 0) s_sum[warp * 16 + g] = l[g];
-      }
-      bar_sync(1, 128);
-#pragma unroll
-      for (int g = 0; g < GP; ++g) l[g] = (s_sum[g] + s_sum[16 + g]) + (s_sum[32 + g] + s_sum[48 + g]);
-      mbar_wait(&pv_done[(it - 1) & 1], ((it - 1) >> 1) & 1, s_abort);
-      __syncwarp();
-      tc_fence_after();
-      uint32_t hi[GP], lo[GP];
-      tmem_ld_n<GP>(tmem + lanes + kColO, hi);
-      tmem_ld_n<GP>(tmem + lanes + kColO + GP, lo);
-      tmem_ld_wait();
+      // ---- the segment's sums: of either group, then of both
       float o[GP];
 #pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        // (an infinite value times a low part, which may be 0 or negative, is none of the formula's terms)
-        const float y = __uint_as_float(lo[g]);
-        o[g] = __uint_as_float(hi[g]) + (fabsf(y) < INFINITY ? y : 0.f);
+      for (int g = 0; g < GP; ++g) o[g] = 0.f;
+      if (last >= 0) {                                     // (the same for the whole group)
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          for (int k = 16; k > 0; k >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], k);
+          if (lane == 0) my_sum[(warp & 3) * 16 + g] = l[g];
+        }
+        bar_sync(2 + grp, 128);
+#pragma unroll
+        for (int g = 0; g < GP; ++g) l[g] = (my_sum[g] + my_sum[16 + g]) + (my_sum[32 + g] + my_sum[48 + g]);
+        mbar_wait(&pv_done[grp], (last >> 1) & 1, s_abort);
+        __syncwarp();
+        tc_fence_after();
+        uint32_t hi[GP], lo[GP];
+        tmem_ld_n<GP>(o_col, hi);
+        tmem_ld_n<GP>(o_col + GP, lo);
+        tmem_ld_wait();
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          // (an infinite value times a low part, which may be 0 or negative, is none of the formula's terms)
+          const float y = __uint_as_float(lo[g]);
+          o[g] = __uint_as_float(hi[g]) + (fabsf(y) < INFINITY ? y : 0.f);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[qslot]);
-      if (d.slot >= 0) {
+      if (grp == 1) {
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          other_o[g * 128 + row] = o[g];
+          if (row == g) s_join[g] = m[g], s_join[16 + g] = l[g];
+        }
+      }
+      bar_sync(1, 256);
+      float lse[GP];
+      if (grp == 0) {
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          const float m1 = s_join[g], top = fmaxf(m[g], m1);
+          const float f0 = exp2_fast(m[g] - top), f1 = exp2_fast(m1 - top);
+          m[g] = top;
+          l[g] = l[g] * f0 + s_join[16 + g] * f1;
+          o[g] = o[g] * f0 + other_o[g * 128 + row] * f1;
+          lse[g] = m[g] + log2f(l[g]);
+          if (row == g) s_join[32 + g] = lse[g];
+        }
+      }
+      bar_sync(1, 256);                                    // group 1's buffer may be written again
+      if (grp == 0) {
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
           if (g >= w.n) continue;
-          if (tid < DH)
-            p.ws_o[(static_cast<int64_t>(d.slot) * GP + g) * DH + tid] = o[g];
-          if (tid == g) p.ws_ml[d.slot * GP + g] = make_float2(m[g], l[g]);
+          if (d.slot >= 0) {
+            if (row < DH) p.ws_o[(static_cast<int64_t>(d.slot) * GP + g) * DH + row] = o[g];
+            if (row == g) p.ws_ml[d.slot * GP + g] = make_float2(m[g], l[g]);
+          } else {
+            if (row < DH) p.out[w.s * p.os[0] + (w.hq0 + g) * p.os[1] + row] = narrow<BF16>(o[g] / l[g]);
+            if (row == g) {
+              if (p.lse != nullptr) p.lse[static_cast<int64_t>(w.s) * p.Hq + w.hq0 + g] = lse[g] * 0.6931471805599453f;
+              if (xs != nullptr) p.ws_lse[static_cast<int64_t>(d.unit) * GP + g] = lse[g];
+            }
+          }
         }
-        continue;
       }
-      float lse[GP];
+      if (xs != nullptr && p.chunks == 1 && d.slot < 0) {
+        // (a thread reads the logits it wrote itself)
+        const int nt = (d.ntok + kTile - 1) / kTile, t_first = ((it - nt) & 1) == grp ? 0 : 1;
+        float le[GP];
 #pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        lse[g] = m[g] + log2f(l[g]);
-        if (g >= w.n) continue;
-        if (tid < DH)
-          p.out[w.s * p.os[0] + (w.hq0 + g) * p.os[1] + tid] = narrow<BF16>(o[g] / l[g]);
-        if (tid == g) {
-          if (p.lse != nullptr) p.lse[static_cast<int64_t>(w.s) * p.Hq + w.hq0 + g] = lse[g] * 0.6931471805599453f;
-          if (xs != nullptr) p.ws_lse[static_cast<int64_t>(d.unit) * GP + g] = lse[g];
-        }
-      }
-      if (xs != nullptr && p.chunks == 1) {
-        for (int t = tid; t < d.ntok; t += 128) {                     // (d.tok0 is 0)
+        for (int g = 0; g < GP; ++g) le[g] = s_join[32 + g];
+        for (int t = t_first * kTile + row; t < d.ntok; t += 2 * kTile) {             // (d.tok0 is 0)
           float add = 0.f;
 #pragma unroll
           for (int g = 0; g < GP; ++g)
-            if (g < w.n) add += exp2_fast(xs[g * p.x_stride + t] - lse[g]);
+            if (g < w.n) add += exp2_fast(xs[g * p.x_stride + t] - le[g]);
           const int pg = paged_page(p.v, w.s, t >> p.v.page_shift);
           if (pg >= 0)
             atomicAdd(p.weights + (static_cast<int64_t>(pg) * p.v.Hkv + w.h) * p.v.page + (t & (p.v.page - 1)), add);
@@ -597,9 +682,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     __nanosleep(1000000);  // let copies and products that are still in flight land before the CTA goes away
     __syncthreads();
   }
-  if (warp == 5) {
+  if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 64);
+    tmem_dealloc(tmem, kTmemColumns);
   }
 }
 
@@ -679,12 +764,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
   int at = static_cast<int>(static_cast<int64_t>(total) * blockIdx.x / gridDim.x);
   const int stop = static_cast<int>(static_cast<int64_t>(total) * (blockIdx.x + 1) / gridDim.x);
   if (at >= stop) return;
-  int lo = 0, hi = p.units;                           // the last unit that begins at or before `at`
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.ws_prefix[mid] <= at) lo = mid;
-    else hi = mid;
-  }
+  __shared__ int s_before[kWarps];                    // units that begin at or before `at`: the last of them holds it
+  int before = 0;
+  for (int u = tid; u < p.units; u += kJoinThreads) before += p.ws_prefix[u] <= at ? 1 : 0;
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) s_before[warp] = before;
+  __syncthreads();
+  int lo = -1;
+  for (int k = 0; k < kWarps; ++k) lo += s_before[k];
   constexpr int kPerThread = 4;
   for (int u = lo; at < stop; ++u) {
     const int a = p.ws_prefix[u], b = p.ws_prefix[u + 1];

@@ -201,8 +201,9 @@ __device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t
       "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__host__ __device__ constexpr uint32_t umma_desc_hi(uint32_t sbo_bytes) {
-  return (sbo_bytes >> 4) | (1u << 14) | (2u << 29);
+// (layout: 2 = 128-byte swizzle, 4 = 64-byte, 6 = 32-byte)
+__host__ __device__ constexpr uint32_t umma_desc_hi(uint32_t sbo_bytes, uint32_t layout = 2) {
+  return (sbo_bytes >> 4) | (1u << 14) | (layout << 29);
 }
 
 // 32 lanes x N consecutive 32-bit columns, N = 1 .. 16: thread i of the warp gets (or gives) lane (base+i).
