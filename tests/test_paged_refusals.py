@@ -91,7 +91,7 @@ def test_workspaces(lib):
 @pytest.mark.parametrize("change,code", [
     (dict(q=None), -1), (dict(out=None), -1), (dict(kv=None), -1), (dict(table=None), -1), (dict(lens=None), -1),
     (dict(Hq=0), -3), (dict(Hq=6), -3), (dict(Hq=65536), -7), (dict(q=FAKE + 8), -2), (dict(q_strides=(4, 8)), -2),
-    (dict(out_strides=(8, -8)), -3)])
+    (dict(out_strides=(8, -8)), -3), (dict(weights=FAKE + 4), -2)])
 def test_bad_attention(lib, change, code):
     assert lib.we_b200_paged_attn(ctypes.byref(attn_args(**change)), None, None) == code
 

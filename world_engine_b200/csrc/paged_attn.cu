@@ -167,6 +167,40 @@ __device__ __forceinline__ int share_of(const PagedAttnParams& p, int total) {
   return max((total + p.grid - 1) / p.grid, p.min_share);
 }
 
+// The pages of a segment's granules, for a warp that loads tiles: 32 granules (four or eight tiles) per look-up of the
+// table, the next 32 under way while these are used.
+struct PageWalk {
+  const int32_t* row;        // the session's table row
+  int next, end, here, ahead;
+
+  __device__ __forceinline__ int fetch(const PagedAttnParams& p, int lane) {
+    const int tok = next + (lane << p.gran_shift);
+    next += 32 << p.gran_shift;
+    return tok < end ? row[tok >> p.v.page_shift] : 0;
+  }
+  __device__ __forceinline__ void begin(const PagedAttnParams& p, int s, int tok0, int tok1, int lane) {
+    row = p.v.table + s * p.v.table_stride;
+    next = tok0;
+    end = tok1;
+    here = fetch(p, lane);
+    ahead = next < end ? fetch(p, lane) : 0;
+  }
+  // The page of granule `lane` of the segment's tile `i`.
+  __device__ __forceinline__ int page(const PagedAttnParams& p, int i, int lane) {
+    const int per = kTile >> p.gran_shift, first = (i * per) & 31;
+    if (first == 0 && i > 0) {
+      here = ahead;
+      ahead = next < end ? fetch(p, lane) : 0;
+    }
+    int pg = __shfl_sync(0xffffffffu, here, first + (lane & (per - 1)));
+    if (pg < 0 || pg >= p.v.n_pages) {
+      paged_report(p.v);
+      pg = 0;
+    }
+    return pg;
+  }
+};
+
 template <int DH, bool BF16, int GP>
 __global__ void __launch_bounds__(kPagedThreads, 1)
 paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams p) {
@@ -189,7 +223,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   uint64_t* pv_done = p_full + kBufs;
   float* s_max = reinterpret_cast<float*>(aux + 384);                 // [2 groups][4 warps][16]
   float* s_sum = s_max + 128;                                         // [2 groups][4 warps][16]
-  float* s_join = s_sum + 128;                                        // group 1's m and l, lse: [3][16]
+  float* s_join = s_sum + 128;                                        // group 1's m and l: [2][16]
   Segment* segs = reinterpret_cast<Segment*>(aux + 1600);
   int* s_plan = reinterpret_cast<int*>(aux + 1600 + kSegs * 16);      // 0 unit, 1 granule, 2 run, 4.. scan
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_plan + 30);
@@ -235,6 +269,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
       s_plan[0] = u0;
       s_plan[1] = 0;
       s_plan[2] = 0x7FFFFFFF;
+      s_plan[3] = u0 < end_unit ? held(u0) : 0;
     }
     for (int u = u0 + tid; u < end_unit; u += kPagedThreads)
       if (held(u) == 0) write_empty(p, u, DH);
@@ -270,6 +305,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
       for (int n = granules(held(u)); at + n <= g0; n = granules(held(++u))) at += n;
       s_plan[0] = u;
       s_plan[1] = static_cast<int>(g0) - at;
+      s_plan[3] = held(u);
     }
     if (cta == 0) {                      // for the join
       int at = pre;
@@ -287,26 +323,25 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   const uint32_t tmem = *s_tmem;
   if (warp == 8) {
     // ---------------------------------------------------------------- K tiles and segments
-    int u = s_plan[0], at = s_plan[1], left = s_plan[2];
+    const uint64_t policy = p.chunks == 1 ? l2_evict_first() : l2_evict_normal();
+    int u = s_plan[0], at = s_plan[1], left = s_plan[2], n = s_plan[3];
     int seg = 0, it = 0;
     bool ok = true;
     while (ok && left > 0 && u < end_unit) {
-      const int n = held(u), tok0 = at << gs;
+      const int n_next = u + 1 < end_unit ? p.lens[(u + 1) / p.chunks] : 0;      // (clamped when its turn comes)
+      const int tok0 = at << gs;
       int ntok = n - tok0;
       if (!p.whole) ntok = static_cast<int>(min(static_cast<int64_t>(ntok), static_cast<int64_t>(left) << gs));
       if (ntok <= 0) {
         ++u;
         at = 0;
+        n = paged_count(p.v, n_next);
         continue;
       }
       const UnitHeads w = unit_heads(p, u);
       const int qslot = seg % kSegs, end = tok0 + ntok, x0 = w.h * static_cast<int>(p.unit_head);
-      auto page_at = [&](int tok) {
-        if (lane >= (kTile >> gs) || tok >= end) return -1;
-        const int pg = paged_page(p.v, w.s, tok >> p.v.page_shift);
-        return pg < 0 ? 0 : pg;
-      };
-      int tok = tok0 + (lane << gs), pg = page_at(tok);
+      PageWalk walk;
+      walk.begin(p, w.s, tok0, end, lane);
       constexpr int kVecs = DH / 8, kLoads = (GP * kVecs + 31) / 32;
       uint4 q[kLoads];
 #pragma unroll
@@ -319,7 +354,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
       ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qslot], ((seg / kSegs) & 1) ^ 1, s_abort));
       for (int t0 = tok0; t0 < end && ok; t0 += kTile, ++it) {
         const int st = it % C::kStages, ng = (min(kTile, end - t0) + (1 << gs) - 1) >> gs;
-        const int next = tok + kTile, pg_next = page_at(next);
+        const int pg = walk.page(p, (t0 - tok0) / kTile, lane);
         ok = mbar_wait(&k_empty[st], ((it / C::kStages) & 1) ^ 1, s_abort);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -327,9 +362,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
         __syncwarp();
         if (lane < ng)
           tma_load_5d(smem_u32(sK + st * C::kTileBytes) + lane * ((DH * 2) << gs), &tm, &k_full[st], 0, 0, 0,
-                      (tok & (p.v.page - 1)) >> 3, pg * static_cast<int>(p.unit_page) + x0);
-        tok = next;
-        pg = pg_next;
+                      ((t0 + (lane << gs)) & (p.v.page - 1)) >> 3, pg * static_cast<int>(p.unit_page) + x0, policy);
         if (t0 == tok0) {
           // the segment's query rows: [chunk][16 rows][128 bytes], 128-byte swizzle
 #pragma unroll
@@ -356,6 +389,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
       if (!p.whole) left -= granules(ntok);
       ++u;
       at = 0;
+      n = paged_count(p.v, n_next);
     }
     if (ok && mbar_wait(&q_empty[seg % kSegs], ((seg / kSegs) & 1) ^ 1, s_abort) && lane == 0) {
       segs[seg % kSegs].ntok = 0;
@@ -363,6 +397,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     }
   } else if (warp == 11) {
     // ---------------------------------------------------------------- V tiles
+    const uint64_t policy = p.chunks == 1 ? l2_evict_first() : l2_evict_normal();
     int it = 0;
     for (int seg = 0;; ++seg) {
       const int qslot = seg % kSegs;
@@ -374,24 +409,18 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
       if (d.ntok == 0) break;
       const UnitHeads w = unit_heads(p, d.unit);
       const int end = d.tok0 + d.ntok, x0 = w.h * static_cast<int>(p.unit_head) + static_cast<int>(p.unit_plane);
-      auto page_at = [&](int tok) {
-        if (lane >= (kTile >> gs) || tok >= end) return -1;
-        const int pg = paged_page(p.v, w.s, tok >> p.v.page_shift);
-        return pg < 0 ? 0 : pg;
-      };
-      int tok = d.tok0 + (lane << gs), pg = page_at(tok);
+      PageWalk walk;
+      walk.begin(p, w.s, d.tok0, end, lane);
       for (int t0 = d.tok0; t0 < end; t0 += kTile, ++it) {
         const int st = it % C::kStages, ng = (min(kTile, end - t0) + (1 << gs) - 1) >> gs;
-        const int next = tok + kTile, pg_next = page_at(next);
+        const int pg = walk.page(p, (t0 - d.tok0) / kTile, lane);
         ok = mbar_wait(&v_empty[st], ((it / C::kStages) & 1) ^ 1, s_abort);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) mbar_arrive_expect_tx(&v_full[st], (ng << gs) * DH * 2);
         __syncwarp();
         if (lane < ng)
           tma_load_5d(smem_u32(sV + st * C::kTileBytes) + lane * ((DH * 2) << gs), &tm, &v_full[st], 0, 0, 0,
-                      (tok & (p.v.page - 1)) >> 3, pg * static_cast<int>(p.unit_page) + x0);
-        tok = next;
-        pg = pg_next;
+                      ((t0 + (lane << gs)) & (p.v.page - 1)) >> 3, pg * static_cast<int>(p.unit_page) + x0, policy);
       }
     }
   } else if (warp == 9) {
@@ -478,6 +507,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
 #pragma unroll
       for (int g = 0; g < GP; ++g) m[g] = kFloor, l[g] = 0.f;
       float* xs = p.weights != nullptr ? p.ws_x + static_cast<int64_t>(d.unit) * GP * p.x_stride + d.tok0 : nullptr;
+      // (the first store to a page the SM has not translated yet holds up everything behind it: ask for it early)
+      if (xs != nullptr && row < w.n) asm volatile("prefetch.global.L2 [%0];" ::"l"(xs + row * p.x_stride));
       int last = -1;                                       // this group's last tile
       for (int t0 = 0; t0 < d.ntok; t0 += kTile, ++it) {
         if ((it & 1) != grp) continue;
@@ -635,7 +666,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
           l[g] = l[g] * f0 + s_join[16 + g] * f1;
           o[g] = o[g] * f0 + other_o[g * 128 + row] * f1;
           lse[g] = m[g] + log2f(l[g]);
-          if (row == g) s_join[32 + g] = lse[g];
         }
       }
       bar_sync(1, 256);                                    // group 1's buffer may be written again
@@ -653,22 +683,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
               if (xs != nullptr) p.ws_lse[static_cast<int64_t>(d.unit) * GP + g] = lse[g];
             }
           }
-        }
-      }
-      if (xs != nullptr && p.chunks == 1 && d.slot < 0) {
-        // (a thread reads the logits it wrote itself)
-        const int nt = (d.ntok + kTile - 1) / kTile, t_first = ((it - nt) & 1) == grp ? 0 : 1;
-        float le[GP];
-#pragma unroll
-        for (int g = 0; g < GP; ++g) le[g] = s_join[32 + g];
-        for (int t = t_first * kTile + row; t < d.ntok; t += 2 * kTile) {             // (d.tok0 is 0)
-          float add = 0.f;
-#pragma unroll
-          for (int g = 0; g < GP; ++g)
-            if (g < w.n) add += exp2_fast(xs[g * p.x_stride + t] - le[g]);
-          const int pg = paged_page(p.v, w.s, t >> p.v.page_shift);
-          if (pg >= 0)
-            atomicAdd(p.weights + (static_cast<int64_t>(pg) * p.v.Hkv + w.h) * p.v.page + (t & (p.v.page - 1)), add);
         }
       }
     }
@@ -758,8 +772,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
     __syncthreads();
   }
   if (p.weights == nullptr) return;
-  // ---- weights of the tokens of this CTA's share of the granules (units that one CTA finished have theirs, unless a
-  // kv head has several units: their shares of a token's weight are added here, in the order of the heads)
+  // ---- weights of the tokens of this CTA's share of the granules; where a kv head has several units, their shares of a
+  // token's weight are added up before they go to memory, in the order of the heads
   const int gs = p.gran_shift;
   int at = static_cast<int>(static_cast<int64_t>(total) * blockIdx.x / gridDim.x);
   const int stop = static_cast<int>(static_cast<int64_t>(total) * (blockIdx.x + 1) / gridDim.x);
@@ -772,48 +786,61 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
   __syncthreads();
   int lo = -1;
   for (int k = 0; k < kWarps; ++k) lo += s_before[k];
-  constexpr int kPerThread = 4;
   for (int u = lo; at < stop; ++u) {
     const int a = p.ws_prefix[u], b = p.ws_prefix[u + 1];
     if (a == b) continue;
     const int from = at - a;
     at = min(b, stop);
-    if (u % p.chunks != 0 || (p.chunks == 1 && pieces_of(a, b, share).n == 1)) continue;
+    if (u % p.chunks != 0) continue;
     const UnitHeads w = unit_heads(p, u);
     const int n = min(paged_count(p.v, p.lens[u / p.chunks]), (at - a) << gs);
-    for (int t0 = from << gs; t0 < n; t0 += kJoinThreads * kPerThread) {
-      float add[kPerThread] = {};
+    for (int t0 = from << gs; t0 < n; t0 += kJoinThreads * 4) {
+      const int t = t0 + 4 * tid;                       // four neighbours: one page, 16 bytes of each head's logits
+      float add[4] = {0.f, 0.f, 0.f, 0.f};
+      const int pg = t < n ? p.v.table[w.s * p.v.table_stride + (t >> p.v.page_shift)] : 0;
       for (int c = 0; c < p.chunks; ++c) {
-        const int ca = p.ws_prefix[u + c];
-        const Pieces r = pieces_of(ca, ca + (b - a), share);
         const int nh = unit_heads(p, u + c).n;
-        __syncthreads();
-        for (int g = warp; g < nh; g += kWarps) {
-          float lse;
-          if (r.n == 1) {
-            lse = p.ws_lse[static_cast<int64_t>(u + c) * GP + g];
-          } else {
-            const float2 ml = join_ml<GP>(p, r, g, lane);
-            lse = ml.x + log2f(ml.y);
-          }
-          if (lane == 0) s_lse[g] = lse;
-        }
-        __syncthreads();
-        const float* xs = p.ws_x + static_cast<int64_t>(u + c) * GP * p.x_stride;
+        const float* xs = p.ws_x + static_cast<int64_t>(u + c) * GP * p.x_stride + t;
+        float4 x[GP];
 #pragma unroll
-        for (int i = 0; i < kPerThread; ++i) {
-          const int t = t0 + i * kJoinThreads + tid;
-          if (t < n)
-            for (int g = 0; g < nh; ++g) add[i] += exp2_fast(xs[g * p.x_stride + t] - s_lse[g]);
+        for (int g = 0; g < GP; ++g)
+          if (t < n && g < nh) x[g] = *reinterpret_cast<const float4*>(xs + g * p.x_stride);
+        if (t0 == from << gs || p.chunks > 1) {
+          const int ca = p.ws_prefix[u + c];
+          const Pieces r = pieces_of(ca, ca + (b - a), share);
+          __syncthreads();
+          for (int g = warp; g < nh; g += kWarps) {
+            float lse;
+            if (r.n == 1) {
+              lse = p.ws_lse[static_cast<int64_t>(u + c) * GP + g];
+            } else {
+              const float2 ml = join_ml<GP>(p, r, g, lane);
+              lse = ml.x + log2f(ml.y);
+            }
+            if (lane == 0) s_lse[g] = lse;
+          }
+          __syncthreads();
+        }
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          if (g >= nh) continue;
+          const float le = s_lse[g];
+          add[0] += exp2_fast(x[g].x - le);
+          add[1] += exp2_fast(x[g].y - le);
+          add[2] += exp2_fast(x[g].z - le);
+          add[3] += exp2_fast(x[g].w - le);
         }
       }
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        const int t = t0 + i * kJoinThreads + tid;
-        if (t >= n) continue;
-        const int pg = paged_page(p.v, w.s, t >> p.v.page_shift);
-        if (pg >= 0)
-          atomicAdd(p.weights + (static_cast<int64_t>(pg) * p.v.Hkv + w.h) * p.v.page + (t & (p.v.page - 1)), add[i]);
+      if (t >= n) continue;
+      if (pg < 0 || pg >= p.v.n_pages) {
+        paged_report(p.v);
+        continue;
+      }
+      float* dst = p.weights + ((static_cast<int64_t>(pg) * p.v.Hkv + w.h) << p.v.page_shift) + (t & (p.v.page - 1));
+      if (t + 3 < n) {
+        atomicAdd(reinterpret_cast<float4*>(dst), make_float4(add[0], add[1], add[2], add[3]));
+      } else {
+        for (int i = 0; t + i < n; ++i) atomicAdd(dst + i, add[i]);
       }
     }
   }
@@ -838,22 +865,17 @@ static int paged_plan(const we_b200_paged_geom& g, int Hq, bool accumulate, Page
   if (units > (1 << 24) || most > 0x3FFFFFFF) return WE_B200_E_LIMIT;
   r->units = static_cast<int>(units);
   r->min_share = kTile >> r->gran_shift;                            // no less than a tile per CTA
-  r->whole = r->cap <= kWholeUnitTokens || r->units == 0;
+  r->whole = r->cap <= kWholeUnitTokens && !accumulate;
   const int64_t want = r->whole ? units : (most + r->min_share - 1) / r->min_share;
   const int sms = sm_count();
   r->grid = static_cast<int>(want < sms ? want : sms);
   auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
-  if (r->whole) {
-    r->off_ml = r->off_o = r->off_lse = 0;
-    r->off_x = up(sizeof(float) * r->units * r->gp);
-  } else {
-    r->off_ml = up(sizeof(int32_t) * (r->units + 1));
-    r->off_o = r->off_ml + up(sizeof(float2) * 2 * r->grid * r->gp);
-    r->off_lse = r->off_o + sizeof(float) * 2 * r->grid * r->gp * g.Dh;
-    r->off_x = r->off_lse + up(sizeof(float) * r->units * r->gp);
-  }
-  r->bytes = accumulate ? r->off_x + sizeof(float) * static_cast<size_t>(r->units) * r->gp * r->cap
-                        : (r->whole ? 0 : r->off_x);
+  r->off_ml = up(sizeof(int32_t) * (r->units + 1));
+  r->off_o = r->off_ml + up(sizeof(float2) * 2 * r->grid * r->gp);
+  r->off_lse = r->off_o + sizeof(float) * 2 * r->grid * r->gp * g.Dh;
+  r->off_x = r->off_lse + up(sizeof(float) * r->units * r->gp);
+  r->bytes = r->whole ? 0 : r->off_x;
+  if (accumulate) r->bytes += sizeof(float) * static_cast<size_t>(r->units) * r->gp * r->cap;
   return WE_B200_OK;
 }
 
@@ -966,7 +988,7 @@ extern "C" int we_b200_paged_attn(const we_b200_paged_attn_args* a, int32_t* sta
     if (a->q_strides[i] < 0 || a->out_strides[i] < 0) return WE_B200_E_SHAPE;
     if ((a->q_strides[i] | a->out_strides[i]) & 7) return WE_B200_E_ALIGN;
   }
-  if (!aligned16(a->q) || !aligned16(a->out) || !aligned16(a->kv)) return WE_B200_E_ALIGN;
+  if (!aligned16(a->q) || !aligned16(a->out) || !aligned16(a->kv) || !aligned16(a->weights)) return WE_B200_E_ALIGN;
   PagedPlan plan;
   if ((rc = paged_plan(g, a->Hq, a->weights != nullptr, &plan)) != WE_B200_OK) return rc;
   if (plan.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < plan.bytes)) return WE_B200_E_WORKSPACE;
