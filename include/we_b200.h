@@ -337,7 +337,7 @@ WE_B200_API int we_b200_paged_append(const we_b200_paged_append_args* args_host,
  * evicted ones left, both in ascending order; the others stay where they are,
  * so little is moved.  What an evicted slot beyond the budget holds is left as
  * it was.  The workspace (we_b200_paged_evict_workspace_bytes) needs no
- * initialisation.
+ * initialisation.  max_pages * page + T < 2^21.
  */
 WE_B200_API int we_b200_paged_append_evict(const we_b200_paged_append_args* args_host, int32_t* status, void* stream);
 WE_B200_API size_t we_b200_paged_evict_workspace_bytes(const we_b200_paged_geom* geom_host, int32_t T, int32_t keep);

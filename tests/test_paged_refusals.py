@@ -73,6 +73,11 @@ def test_bad_budgets(lib, change, code):
     assert lib.we_b200_paged_append_evict(ctypes.byref(append_args(**change)), None, None) == code
 
 
+def test_a_table_too_wide_for_a_budget(lib):
+    g = geom(max_pages=1 << 16, table_stride=1 << 16)
+    assert lib.we_b200_paged_append_evict(ctypes.byref(append_args(g)), None, None) == -7
+
+
 def test_workspaces(lib):
     # a table much wider than the budget: the lists of a session that holds that much need room
     g = geom(max_pages=4096, table_stride=4096)

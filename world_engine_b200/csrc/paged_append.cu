@@ -5,7 +5,7 @@
 // under way before the first store.
 //
 // Under a budget the cluster first finds the key of the last token to keep: weights are mapped to unsigned numbers of
-// the same order (shielded tokens above all) and the keep-th largest is found eight bits at a time, each CTA counting
+// the same order (shielded tokens above all) and the keep-th largest is found digit by digit, each CTA counting
 // the digits of its slice of the candidates and adding up the other CTAs' counts through cluster shared memory.  One
 // pass over weights and positions in global memory; the later passes read keys from shared memory (slices that do not
 // fit are recomputed from global memory).  Then each CTA lists, in the order of the indexes, the holes of its slice
@@ -17,6 +17,10 @@ namespace we {
 
 constexpr int kAppendThreads = 256;
 constexpr int kMaxCluster = 8;
+// Candidates a CTA deals with before its (session, head) gets a cluster: a barrier of the cluster and the counts read
+// through it cost about 2 us a digit, 4096 more candidates in one CTA less (16 heads of 4097: 12.9 us in one CTA,
+// 14.3 in two; 16 heads of 17001: 20.9 us in four CTAs, 28 in eight, which do not all find room at once).
+constexpr int kEvictPerCta = 8192;
 
 struct PagedAppendParams {
   PagedView v;
@@ -34,6 +38,7 @@ struct PagedAppendParams {
   const float* w_new;
   int32_t* ws;           // lists of slices that do not fit in shared memory
   int64_t ws_stride;     // entries of one list of one CTA
+  int64_t ws_chunk;      // entries of everything of one CTA
   int32_t T, keep, sink, recent;
   int32_t vec_shift;     // log2 of 16-byte vectors per row
   int32_t cluster;       // CTAs per (session, head)
@@ -153,9 +158,6 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Page
 }
 
 // ------------------------------------------------------------------ under a budget
-constexpr int kEvictThreads = 512;
-constexpr int kEvictWarps = kEvictThreads / 32;
-
 // Weights as unsigned numbers of the same order: NaN above every number, shielded tokens above NaN, -0 equal to 0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (w != w) return 0xFFFFFFFEu;
@@ -163,18 +165,53 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-__global__ void __launch_bounds__(kEvictThreads) paged_append_evict_kernel(const PagedAppendParams p) {
+// Three digits of 11, 11 and 10 bits.  (Of 8 bits there are four: with the cluster's barrier and the search in every
+// pass that took 1 to 2 us more per call; most weights differ within the first two digits of 11.)
+constexpr int kPasses = 3, kBins = 2048;
+__host__ __device__ constexpr int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__host__ __device__ constexpr uint32_t digit_mask(int pass) { return pass == 2 ? 1023u : 2047u; }
+
+// Sum of x over the threads before this one; *all gets the sum over the block.  (One copy for all its uses: a call of
+// this kernel is a few microseconds, and fetching code that runs once is a part of that.)
+template <int kThreads>
+__device__ __noinline__ uint64_t block_scan(uint64_t x, uint64_t* s_warp, uint64_t* all) {
+  constexpr int kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  uint64_t upto = x;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += y;
+  }
+  __syncthreads();                                       // (s_warp may still be read from the call before)
+  if (lane == 31) s_warp[wid] = upto;
+  __syncthreads();
+  uint64_t w = lane < kWarps ? s_warp[lane] : 0;
+#pragma unroll
+  for (int d = 1; d < kWarps; d <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, w, d);
+    if (lane >= d) w += y;
+  }
+  *all = __shfl_sync(0xffffffffu, w, kWarps - 1);
+  const uint64_t before = __shfl_sync(0xffffffffu, w, wid > 0 ? wid - 1 : 0);
+  return upto - x + (wid > 0 ? before : 0);
+}
+
+template <int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) paged_append_evict_kernel(const PagedAppendParams p) {
+  constexpr int kWarps = kThreads / 32, kOwn = kBins / kThreads;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  extern __shared__ uint32_t s_keys[];                 // [fit] keys, [fit] holes, [fit] movers
-  __shared__ uint32_t s_hist[4][256], s_bins[256];
-  __shared__ int s_count[3][kEvictWarps];
+  extern __shared__ __align__(16) uint32_t s_keys[];   // [fit] keys, holes, movers, [fit / 32] twice: bits
+  __shared__ __align__(16) uint32_t s_hist[kPasses][kBins];
+  __shared__ uint64_t s_warp[32];
+  __shared__ uint32_t s_found[3];                      // digit, how many of it are kept, how many there are
   __shared__ int s_equal, s_lists[3];                  // of this CTA: equal keys; holes, movers, new ones in place
   __shared__ int s_base[3][kMaxCluster + 1];
   const int unit = blockIdx.x / p.cluster, rank = blockIdx.x - unit * p.cluster;
   const int s = unit / p.v.Hkv, h = unit - s * p.v.Hkv;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  for (int b = tid; b < 4 * 256; b += kEvictThreads) s_hist[0][b] = 0;
+  for (int b = tid; b < kPasses * kBins / 4; b += kThreads) reinterpret_cast<uint4*>(s_hist)[b] = make_uint4(0u, 0u, 0u, 0u);
   const int len = paged_count(p.v, p.lens[unit]);
   const int pos0 = p.next_pos[unit];
   const int n = new_count(p, s);
@@ -182,7 +219,7 @@ __global__ void __launch_bounds__(kEvictThreads) paged_append_evict_kernel(const
   const int64_t end = static_cast<int64_t>(pos0) + n;
   __syncthreads();
   if (total <= p.keep) {
-    move_tokens<2>(p, s, h, len, pos0, n, rank * kEvictThreads + tid, p.cluster * kEvictThreads,
+    move_tokens<2>(p, s, h, len, pos0, n, rank * kThreads + tid, p.cluster * kThreads,
                    [&](int e, int* src, int* dst) { *src = *dst = len + e; });
   } else {
     // ---- keys of this CTA's slice, four neighbours at a time (they lie in one page), with the first digit's counts
@@ -199,173 +236,205 @@ __global__ void __launch_bounds__(kEvictThreads) paged_append_evict_kernel(const
       const int64_t m = meta_index(p, pg, h, i & (p.v.page - 1));
       return key_of(p.weights[m], p.positions[m]);
     };
-    auto key = [&](int i) { return fits ? s_keys[i - lo] : key_at(i); };
-    constexpr int kDepth = 4;
-    for (int i0 = lo + 4 * tid; i0 < hi; i0 += 4 * kEvictThreads * kDepth) {
+    // four neighbours from index i on (lo + a multiple of 4); those behind the slice read as 0
+    auto keys4 = [&](int i) -> uint4 {
+      if (fits) return *reinterpret_cast<const uint4*>(s_keys + (i - lo));
+      uint4 k;
+      k.x = i < hi ? key_at(i) : 0u;
+      k.y = i + 1 < hi ? key_at(i + 1) : 0u;
+      k.z = i + 2 < hi ? key_at(i + 2) : 0u;
+      k.w = i + 3 < hi ? key_at(i + 3) : 0u;
+      return k;
+    };
+    constexpr int kDepth = 2;
+    for (int i0 = lo + 4 * tid; i0 < hi; i0 += 4 * kThreads * kDepth) {
       int pg[kDepth];
       float4 w[kDepth];
       int4 pos[kDepth];
 #pragma unroll
       for (int d = 0; d < kDepth; ++d) {
-        const int i = i0 + 4 * kEvictThreads * d;
-        pg[d] = i < hi && i + 3 < len ? paged_page(p.v, s, i >> p.v.page_shift) : -1;
+        const int i = i0 + 4 * kThreads * d;
+        pg[d] = i < hi && i + 3 < len ? p.v.table[s * p.v.table_stride + (i >> p.v.page_shift)] : -1;
       }
 #pragma unroll
       for (int d = 0; d < kDepth; ++d) {
-        if (pg[d] < 0) continue;
-        const int64_t m = meta_index(p, pg[d], h, (i0 + 4 * kEvictThreads * d) & (p.v.page - 1));
+        if (pg[d] < 0 || pg[d] >= p.v.n_pages) continue;
+        const int64_t m = meta_index(p, pg[d], h, (i0 + 4 * kThreads * d) & (p.v.page - 1));
         w[d] = *reinterpret_cast<const float4*>(p.weights + m);
         pos[d] = *reinterpret_cast<const int4*>(p.positions + m);
       }
 #pragma unroll
       for (int d = 0; d < kDepth; ++d) {
-        const int i = i0 + 4 * kEvictThreads * d;
+        const int i = i0 + 4 * kThreads * d;
         if (i >= hi) continue;
         uint32_t k[4];
-        if (pg[d] >= 0) {
+        if (pg[d] >= 0 && pg[d] < p.v.n_pages) {
           k[0] = key_of(w[d].x, pos[d].x);
           k[1] = key_of(w[d].y, pos[d].y);
           k[2] = key_of(w[d].z, pos[d].z);
           k[3] = key_of(w[d].w, pos[d].w);
-        } else {
+        } else {                                        // new tokens, the last held ones, a bad page (reported)
 #pragma unroll
           for (int u = 0; u < 4; ++u) k[u] = i + u < hi ? key_at(i + u) : 0u;
         }
         if (fits) *reinterpret_cast<uint4*>(s_keys + (i - lo)) = make_uint4(k[0], k[1], k[2], k[3]);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          if (i + u < hi) atomicAdd(&s_hist[0][k[u] >> 24], 1u);
+          if (i + u < hi) atomicAdd(&s_hist[0][k[u] >> digit_shift(0)], 1u);
       }
     }
     // ---- the key of the last one kept (its leading digits, as far as they decide), how many of that key are kept
     uint32_t prefix = 0, mask = 0, need = static_cast<uint32_t>(p.keep), equals = 0;
-    for (int pass = 0; pass < 4; ++pass) {
-      const int shift = 24 - 8 * pass;
+#pragma unroll 1
+    for (int pass = 0; pass < kPasses; ++pass) {
+      const int shift = digit_shift(pass);
+      const uint32_t bits = digit_mask(pass);
       if (pass > 0) {
-        for (int i = lo + tid; i < hi; i += kEvictThreads) {
-          const uint32_t k = key(i);
-          if ((k & mask) == prefix) atomicAdd(&s_hist[pass][(k >> shift) & 255u], 1u);
+        for (int i = lo + 4 * tid; i < hi; i += 4 * kThreads) {
+          const uint4 k4 = keys4(i);
+          const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (i + u < hi && (k[u] & mask) == prefix) atomicAdd(&s_hist[pass][(k[u] >> shift) & bits], 1u);
         }
       }
       unit_sync(p);
-      if (p.cluster > 1) {
-        if (tid < 256) {
-          uint32_t x = 0;
-          for (int r = 0; r < p.cluster; ++r) x += of_rank(&s_hist[pass][tid], r)[0];
-          s_bins[tid] = x;
-        }
-        __syncthreads();
-      }
-      // every warp finds the digit for itself: eight bins per lane, the largest digits in lane 0
-      const uint32_t* bins = p.cluster > 1 ? s_bins : s_hist[pass];
-      uint32_t c[8], sum = 0;
+      // kOwn bins per thread, the largest digits in thread 0; a scan over the block finds the one with the keep-th
+      uint32_t c[kOwn], sum = 0;
+      const int bin0 = kBins - kOwn * (tid + 1);
 #pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        c[b] = bins[255 - 8 * lane - b];
-        sum += c[b];
+      for (int b = 0; b < kOwn; ++b) c[b] = 0;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        if (r >= p.cluster) break;
+        const uint32_t* from = p.cluster == 1 ? &s_hist[pass][bin0] : of_rank(&s_hist[pass][bin0], r);
+        if constexpr (kOwn == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(from);
+          c[0] += x.x;
+          c[1] += x.y;
+        } else {
+#pragma unroll
+          for (int b = 0; b < kOwn; b += 4) {
+            const uint4 x = *reinterpret_cast<const uint4*>(from + b);
+            c[b] += x.x;
+            c[b + 1] += x.y;
+            c[b + 2] += x.z;
+            c[b + 3] += x.w;
+          }
+        }
       }
-      uint32_t before = sum;
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, before, d);
-        if (lane >= d) before += y;
-      }
-      before -= sum;
-      const uint32_t who = __ballot_sync(0xffffffffu, before < need && before + sum >= need);
-      uint32_t digit = 0, left = 0, same = 0;
-      {
+#pragma unroll
+      for (int b = 0; b < kOwn; ++b) sum += c[b];
+      uint64_t all;
+      const uint32_t before = static_cast<uint32_t>(block_scan<kThreads>(sum, s_warp, &all));
+      if (before < need && before + sum >= need) {
         uint32_t at = before;
         bool found = false;
 #pragma unroll
-        for (int b = 0; b < 8; ++b) {
+        for (int b = kOwn - 1; b >= 0; --b) {
           if (!found && at + c[b] >= need) {
             found = true;
-            digit = 255 - 8 * lane - b;
-            left = need - at;
-            same = c[b];
+            s_found[0] = bin0 + b;
+            s_found[1] = need - at;
+            s_found[2] = c[b];
           }
           at += c[b];
         }
       }
-      const int from = __ffs(who) - 1;
-      digit = __shfl_sync(0xffffffffu, digit, from);
-      need = __shfl_sync(0xffffffffu, left, from);
-      equals = __shfl_sync(0xffffffffu, same, from);
-      prefix |= digit << shift;
-      mask |= 255u << shift;
+      __syncthreads();
+      prefix |= s_found[0] << shift;
+      mask |= bits << shift;
+      need = s_found[1];
+      equals = s_found[2];
       if (equals == need) break;                         // everything with these digits stays
-      __syncthreads();                                   // (s_bins is read before the next pass writes it)
     }
-    // ---- ranks among equal keys, where not all of them stay: in the order of the indexes
-    const int sub = ((mine + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
-    const int w_lo = min(lo + wid * sub, hi), w_hi = min(w_lo + sub, hi);
-    const uint32_t below = (1u << lane) - 1u;
-    uint32_t equal_base = 0;
-    if (equals != need) {
-      int cnt = 0;
-      for (int i = w_lo; i < w_hi; i += 32)
-        cnt += __popc(__ballot_sync(0xffffffffu, i + lane < w_hi && (key(i + lane) & mask) == prefix));
-      if (lane == 0) s_count[0][wid] = cnt;
-      __syncthreads();
-      if (tid == 0) {
-        int x = 0;
-        for (int w = 0; w < kEvictWarps; ++w) x += s_count[0][w];
-        s_equal = x;
-      }
-      unit_sync(p);
-      for (int r = 0; r < rank; ++r) equal_base += *of_rank(&s_equal, r);
-      for (int w = 0; w < wid; ++w) equal_base += s_count[0][w];
-      __syncthreads();
-    }
-    // ---- holes, movers and new tokens that lie below the budget already: counted, then listed
-    int32_t* holes = fits ? reinterpret_cast<int32_t*>(s_keys) + p.fit
-                          : p.ws + (static_cast<int64_t>(blockIdx.x) * 2) * p.ws_stride;
-    int32_t* movers = holes + (fits ? p.fit : p.ws_stride);
+    // ---- one bit per candidate: kept outright, or one of the equal keys of which only some are kept
+    int32_t* holes = fits ? reinterpret_cast<int32_t*>(s_keys) + p.fit : p.ws + blockIdx.x * p.ws_chunk;
     const int64_t room = fits ? p.fit : p.ws_stride;
-    int at[3] = {0, 0, 0};
-    for (int round = 0; round < 2; ++round) {
-      uint32_t rank_eq = equal_base;
-      for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
-        const int i = i0 + lane;
-        const bool in = i < w_hi;
-        const uint32_t k = in ? key(i) & mask : 0u;
-        const bool equal = in && k == prefix;
-        bool kept = in && (k > prefix || equal);
-        if (equals != need) {
-          const uint32_t e = __ballot_sync(0xffffffffu, equal);
-          if (equal && rank_eq + __popc(e & below) >= need) kept = false;
-          rank_eq += __popc(e);
-        }
-        const bool hole = in && i < p.keep && !kept, mover = kept && i >= p.keep, stay = kept && i >= len && i < p.keep;
-        const uint32_t b0 = __ballot_sync(0xffffffffu, hole), b1 = __ballot_sync(0xffffffffu, mover),
-                       b2 = __ballot_sync(0xffffffffu, stay);
-        if (round == 1) {
-          if (hole) holes[at[0] + __popc(b0 & below)] = i;
-          if (mover) movers[at[1] + __popc(b1 & below)] = i;
-          if (stay) holes[room - 1 - (at[2] + __popc(b2 & below))] = i;      // from the far end
-        }
-        at[0] += __popc(b0);
-        at[1] += __popc(b1);
-        at[2] += __popc(b2);
+    int32_t* movers = holes + room;
+    uint32_t* bits_kept = reinterpret_cast<uint32_t*>(movers + room);
+    uint32_t* bits_equal = bits_kept + ((room + 31) >> 5);
+    const bool ties = equals != need;
+    const int words = (mine + 31) >> 5;
+#pragma unroll 2
+    for (int w = wid; w < words; w += kWarps) {
+      const int i = lo + 32 * w + lane;
+      const uint32_t k = i < hi ? (fits ? s_keys[i - lo] : key_at(i)) & mask : 0u;
+      const uint32_t more = __ballot_sync(0xffffffffu, i < hi && k > prefix);
+      const uint32_t same = __ballot_sync(0xffffffffu, i < hi && k == prefix);
+      if (lane == 0) {
+        bits_kept[w] = ties ? more : more | same;
+        bits_equal[w] = same;
       }
-      if (round == 1) break;
-      if (lane < 3) s_count[lane][wid] = lane == 0 ? at[0] : lane == 1 ? at[1] : at[2];
-      __syncthreads();
-#pragma unroll
-      for (int q = 0; q < 3; ++q) {
-        int x = 0;
-        for (int w = 0; w < wid; ++w) x += s_count[q][w];
-        if (wid == kEvictWarps - 1 && lane == 0) s_lists[q] = x + at[q];
-        at[q] = x;
+    }
+    __syncthreads();
+    // a thread goes on with `per` neighbouring words
+    const int per = (words + kThreads - 1) / kThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
+    if (ties) {                                          // the first `need` of them, in the order of the indexes
+      uint32_t cnt = 0;
+      for (int w = w0; w < w1; ++w) cnt += __popc(bits_equal[w]);
+      uint64_t all;
+      int64_t left = need;
+      left -= static_cast<int64_t>(block_scan<kThreads>(cnt, s_warp, &all));
+      if (p.cluster > 1) {
+        if (tid == 0) s_equal = static_cast<int>(all);
+        unit_sync(p);
+        left -= __reduce_add_sync(0xffffffffu, lane < rank ? *of_rank(&s_equal, lane) : 0);
       }
+      for (int w = w0; w < w1; ++w) {
+        uint32_t e = bits_equal[w];
+        const int have = __popc(e);
+        for (int drop = have - static_cast<int>(left < 0 ? 0 : left < have ? left : have); drop > 0; --drop)
+          e &= ~(0x80000000u >> __clz(e));
+        bits_kept[w] |= e;
+        left -= have;
+      }
+    }
+    // ---- holes, movers and new tokens that lie below the budget already, listed in the order of the indexes
+    auto bits_from = [&](int base, int from) {           // bits of the word at `base` whose index is >= from
+      const int d = from - base;
+      return d <= 0 ? 0xFFFFFFFFu : d >= 32 ? 0u : 0xFFFFFFFFu << d;
+    };
+    auto split = [&](int w, uint32_t* hole, uint32_t* mover, uint32_t* stay) {
+      const int base = lo + 32 * w;
+      const uint32_t kept = bits_kept[w], in = ~bits_from(base, hi), beyond = bits_from(base, p.keep);
+      *hole = ~kept & in & ~beyond;
+      *mover = kept & beyond;
+      *stay = kept & ~beyond & bits_from(base, len);
+    };
+    uint64_t sums = 0;                                   // 21 bits each
+    for (int w = w0; w < w1; ++w) {
+      uint32_t b[3];
+      split(w, &b[0], &b[1], &b[2]);
+      sums += static_cast<uint64_t>(__popc(b[0])) | (static_cast<uint64_t>(__popc(b[1])) << 21) |
+              (static_cast<uint64_t>(__popc(b[2])) << 42);
+    }
+    uint64_t all;
+    const uint64_t at = block_scan<kThreads>(sums, s_warp, &all);
+    int64_t at_h = at & 0x1FFFFF, at_m = (at >> 21) & 0x1FFFFF, at_s = at >> 42;
+    if (tid == 0) {
+      s_lists[0] = static_cast<int>(all & 0x1FFFFF);
+      s_lists[1] = static_cast<int>((all >> 21) & 0x1FFFFF);
+      s_lists[2] = static_cast<int>(all >> 42);
+    }
+    for (int w = w0; w < w1; ++w) {
+      uint32_t b[3];
+      split(w, &b[0], &b[1], &b[2]);
+      const int base = lo + 32 * w;
+      for (; b[0] != 0; b[0] &= b[0] - 1) holes[at_h++] = base + __ffs(b[0]) - 1;
+      for (; b[1] != 0; b[1] &= b[1] - 1) movers[at_m++] = base + __ffs(b[1]) - 1;
+      for (; b[2] != 0; b[2] &= b[2] - 1) holes[room - 1 - at_s++] = base + __ffs(b[2]) - 1;     // from the far end
     }
     unit_sync(p);
-    if (tid < 3) {
-      int x = 0;
-      for (int r = 0; r < p.cluster; ++r) {
-        s_base[tid][r] = x;
-        x += of_rank(&s_lists[tid], r)[0];
+    if (wid < 3) {                                       // where each CTA's entries begin
+      const int x = lane < p.cluster ? (p.cluster == 1 ? s_lists[wid] : *of_rank(&s_lists[wid], lane)) : 0;
+      int upto = x;
+      for (int d = 1; d < kMaxCluster; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += y;
       }
-      for (int r = p.cluster; r <= kMaxCluster; ++r) s_base[tid][r] = x;
+      if (lane < kMaxCluster) s_base[wid][lane + 1] = upto;
+      if (lane == 0) s_base[wid][0] = 0;
     }
     __syncthreads();
     // ---- the moves, spread over the cluster
@@ -374,10 +443,10 @@ __global__ void __launch_bounds__(kEvictThreads) paged_append_evict_kernel(const
       int r = 0;
       while (r + 1 < p.cluster && j >= s_base[q][r + 1]) ++r;
       const int64_t k = q == 2 ? room - 1 - (j - s_base[q][r]) : j - s_base[q][r];
-      if (fits) return of_rank(list, r)[k];
-      return list[static_cast<int64_t>(r - rank) * 2 * p.ws_stride + k];
+      if (fits) return p.cluster == 1 ? list[k] : of_rank(list, r)[k];
+      return list[static_cast<int64_t>(r - rank) * p.ws_chunk + k];
     };
-    move_tokens<2>(p, s, h, len, pos0, moves + stays, rank * kEvictThreads + tid, p.cluster * kEvictThreads,
+    move_tokens<2>(p, s, h, len, pos0, moves + stays, rank * kThreads + tid, p.cluster * kThreads,
                    [&](int e, int* src, int* dst) {
                      if (e < moves) {
                        *src = entry(1, movers, e);
@@ -427,7 +496,7 @@ static int fill(const we_b200_paged_append_args* a, int32_t* status, PagedAppend
   p->n_new = a->n_new;
   p->w_new = a->w_new;
   p->ws = nullptr;
-  p->ws_stride = 0;
+  p->ws_stride = p->ws_chunk = 0;
   p->cluster = 1;
   p->fit = 0;
   p->T = a->T;
@@ -468,24 +537,48 @@ static int cluster_for(int64_t units, int64_t work, int64_t per_cta, int64_t mos
 }
 
 struct EvictPlan {
-  int cluster, fit;
-  int64_t list;            // entries of a list in the workspace, 0: never needed
+  int threads, cluster, fit;
+  int64_t list, chunk;     // entries of a list in the workspace (0: never needed) and of all a CTA has there
   size_t bytes;
 };
-constexpr int kMaxFit = 16384;        // 12 bytes each of the 227 KB
+constexpr int kMaxFit = 16384;
+constexpr int evict_smem(int fit) { return 12 * fit + 2 * ((fit + 31) / 32) * 4; }
+static_assert(evict_smem(kMaxFit) + kPasses * kBins * 4 + 1024 <= 227 * 1024, "shared memory");
 
 // (the counts are on the device: a session that holds more than its budget says, once, is found there)
 static EvictPlan evict_plan(const we_b200_paged_geom& g, int32_t T, int32_t keep) {
   EvictPlan r;
   const int64_t units = static_cast<int64_t>(g.S) * g.Hkv, usual = static_cast<int64_t>(keep) + T;
-  r.cluster = cluster_for(units, usual, 1024, 4 * sm_count());
-  const int64_t fit = ((usual + r.cluster - 1) / r.cluster + 1027) & ~3ll;
+  // four CTAs of 256 threads fit on an SM, or one of 512 has it to itself (one head of 4097: 15.5 us with 256 threads,
+  // 12.9 with 512, 13.6 with 1024, whose scans over the block take longer; 512 heads of 2064: 13.5 us, 16.4 with 512)
+  r.threads = units > 2 * sm_count() ? 256 : 512;
+  r.cluster = cluster_for(units, usual, kEvictPerCta, sm_count());
+  const int64_t fit = ((usual + r.cluster - 1) / r.cluster + 3) & ~3ll;
   r.fit = static_cast<int>(fit < kMaxFit ? fit : kMaxFit);
   const int64_t most = static_cast<int64_t>(g.max_pages) * g.page + T;
   const int64_t slice = ((most + r.cluster - 1) / r.cluster + 3) & ~3ll;
   r.list = slice <= r.fit ? 0 : slice;
-  r.bytes = static_cast<size_t>(units) * r.cluster * 2 * r.list * sizeof(int32_t);
+  r.chunk = 2 * r.list + 2 * ((r.list + 31) >> 5);
+  r.bytes = static_cast<size_t>(units) * r.cluster * r.chunk * sizeof(int32_t);
   return r;
+}
+
+template <int kThreads>
+static int launch_evict(const PagedAppendParams& p, cudaStream_t stream) {
+  static std::atomic<bool> done[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  if (dev < 0 || dev >= kMaxDevices) return WE_B200_E_LIMIT;
+  if (!done[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(paged_append_evict_kernel<kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, evict_smem(kMaxFit));
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return static_cast<int>(e);
+    }
+    done[dev].store(true, std::memory_order_release);
+  }
+  return launch(paged_append_evict_kernel<kThreads>, p, kThreads, evict_smem(p.fit), stream);
 }
 
 }  // namespace we
@@ -512,29 +605,20 @@ extern "C" int we_b200_paged_append_evict(const we_b200_paged_append_args* a, in
   if (a->keep < 1 || a->sink < 0 || a->recent < 0) return WE_B200_E_SHAPE;
   if (static_cast<int64_t>(a->sink) + a->recent > a->keep) return WE_B200_E_SHAPE;
   if (static_cast<int64_t>(a->geom.max_pages) * a->geom.page < a->keep) return WE_B200_E_SHAPE;
+  // (a CTA counts its holes and movers in 21 bits)
+  if (static_cast<int64_t>(a->geom.max_pages) * a->geom.page + a->T >= (1 << 21)) return WE_B200_E_LIMIT;
   const we::EvictPlan plan = we::evict_plan(a->geom, a->T, a->keep);
   if (plan.bytes > 0 && (a->workspace == nullptr || a->workspace_bytes < plan.bytes)) return WE_B200_E_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a->workspace) & 3u) return WE_B200_E_ALIGN;
   if ((reinterpret_cast<uintptr_t>(a->weights) | reinterpret_cast<uintptr_t>(a->positions)) & 15u) return WE_B200_E_ALIGN;
   p.ws = static_cast<int32_t*>(a->workspace);
   p.ws_stride = plan.list;
+  p.ws_chunk = plan.chunk;
   p.keep = a->keep;
   p.sink = a->sink;
   p.recent = a->recent;
   p.cluster = plan.cluster;
   p.fit = plan.fit;
-  static std::atomic<bool> done[we::kMaxDevices];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  if (dev < 0 || dev >= we::kMaxDevices) return WE_B200_E_LIMIT;
-  if (!done[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(we::paged_append_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 12 * we::kMaxFit);
-    if (e != cudaSuccess) {
-      (void)cudaGetLastError();
-      return static_cast<int>(e);
-    }
-    done[dev].store(true, std::memory_order_release);
-  }
-  return we::launch(we::paged_append_evict_kernel, p, we::kEvictThreads, 12 * plan.fit, static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return plan.threads == 256 ? we::launch_evict<256>(p, st) : we::launch_evict<512>(p, st);
 }
