@@ -59,7 +59,24 @@ def test_attention_of_long_and_ragged_batches(S, H, G, lens, accumulate):
     before = c.w64.copy()
     lse = torch.empty(S, H * G, device="cuda")
     out = ops.paged_attn(q, c.kv, c.table, c.lens, weights=c.weights if accumulate else None, lse=lse)
-    check_attention(c, q, out, lse, before, c.weights)if accumulate else check_attention(c, q, out, lse)
+    check_attention(c, q, out, lse, before, c.weights if accumulate else None)
+
+
+@pytest.mark.parametrize("S,H,G,page,lens", [
+    (5, 16, 1, 64, [8192, 8000, 8191, 7777, 8100]),          # long runs: their ends are handed out one by one
+    (9, 5, 20, 16, [8192, 6000, 0, 8191, 7001, 1, 8180, 8100, 7900]),   # ... with two units per kv head
+    (2, 3, 4, 32, [120001, 119000])])
+def test_attention_where_runs_are_handed_out(S, H, G, page, lens):
+    c = Cache(S, H, 64, page, -(-max(lens) // page), BF16, seed=S, lens=lens)
+    q = queries(c, G)
+    before = c.w64.copy()
+    out = ops.paged_attn(q, c.kv, c.table, c.lens, weights=c.weights)
+    check_attention(c, q, out, None, before, c.weights)
+    first = c.weights.clone()
+    for _ in range(3):                                       # whoever takes a run, the result is the same
+        c.weights.copy_(torch.from_numpy(c.w64).float())
+        assert torch.equal(ops.paged_attn(q, c.kv, c.table, c.lens, weights=c.weights), out)
+        assert torch.equal(c.weights.nan_to_num(), first.nan_to_num())
 
 
 @pytest.mark.parametrize("gain", [0.0, 8.0, 40.0])

@@ -8,10 +8,11 @@
 // columns, so K (K-major) and V (MN-major) are read as they lie in shared memory.
 //
 // Work is cut by tokens, not by heads: the tokens of all (session, kv head, chunk of 16 query heads) units are laid end
-// to end in granules of 16 or 32 tokens and every CTA gets an equal run of them, whatever the sessions' lengths, so
-// all SMs finish together.  A run crosses units: each piece is a segment, with its own softmax statistics.  A unit that
-// lies in one CTA is finished there; of one that several CTAs share each leaves (m, l, O) in the workspace and
-// paged_join_kernel puts them together, in the order of the tokens.
+// to end in granules of 16 or 32 tokens and cut into equal runs, one per CTA, whatever the sessions' lengths.  The SMs
+// do not read equally fast (runs of one length end up to 12% apart), so of long runs a part is cut off into small
+// pieces that the CTAs which finish first take one by one.  A run crosses units: each part is a segment, with its own
+// softmax statistics.  A unit that lies in one run is finished there; of one that lies in several each leaves
+// (m, l, O) in the workspace and paged_join_kernel puts them together, in the order of the tokens.
 //
 // One CTA per SM, 384 threads:
 //   warps 0-7  softmax, two groups of 128 threads that take tiles in turn, each with statistics and an accumulator of
@@ -22,8 +23,9 @@
 //              columns: the second column costs nothing (N is at least 16) and leaves the weights accurate to 2^-16
 //              instead of 2^-8.  A token's columns lie next to each other (P is an MN-major operand): one or two
 //              16-byte stores per token.
-//   warp 8     K: walks the run, publishes the segments with their Q rows, loads the K tiles
-//   warp 11    V tiles (a ring of its own)
+//   warp 8     walks the run and publishes the segments, one ahead of the one being loaded: what to read, its first
+//              pages, its Q rows; takes further runs
+//   warp 11    loads the K and V tiles (a ring each)
 //   warp 9     issues S^T, warp 10 issues O^T (one thread each)
 // Tensor memory (128 columns): four S buffers of 16, O of either group (high and low parts of up to 16 heads: 32).
 #include <cuda_bf16.h>
@@ -38,7 +40,7 @@ namespace we {
 constexpr int kPagedThreads = 384;
 constexpr int kPagedWarps = kPagedThreads / 32;
 constexpr int kTile = 128;                 // tokens per tile
-constexpr int kSegs = 4;                   // segments in flight
+constexpr int kSegs = 3;                   // segments in flight
 constexpr int kBufs = 4;                   // S buffers
 constexpr uint32_t kTmemColumns = 128;
 constexpr uint32_t kColO = 64;             // + 32 per group
@@ -57,9 +59,9 @@ struct PagedAttnParams {
   float* weights;
   float* lse;
   // workspace
-  int32_t* ws_prefix;        // [units + 1] granules before a unit
-  float2* ws_ml;             // [2 grid][GP] statistics of the segments of shared units
-  float* ws_o;               // [2 grid][GP][DH]
+  int32_t* ws_prefix;        // [units + 1] granules before a unit; then the number of small runs handed out
+  float2* ws_ml;             // [2 runs][GP] statistics of the segments of shared units
+  float* ws_o;               // [2 runs][GP][DH]
   float* ws_lse;             // [units][GP] log2 of the softmax sum of units one CTA finished
   float* ws_x;               // [units][GP][cap] logits (log2 units)
   int64_t x_stride;          // max_pages * page
@@ -68,7 +70,10 @@ struct PagedAttnParams {
   int32_t units, grid;
   int32_t gran_shift;        // log2 of the tokens per granule
   int32_t whole;             // 1: every unit belongs to one CTA (no join)
-  int32_t min_share;         // granules a CTA gets at least
+  int32_t min_share;         // granules of a tile: what a CTA gets at least, and what beginning a unit counts
+  int32_t dynamic;           // 1: long runs are shortened, and the rest handed out
+  int32_t out_blocks;        // join: CTAs that join outputs (the others give the tokens their weights)
+  int32_t out_by_warp;       // join: 1: a head per warp
   float scale_log2;
 };
 
@@ -133,8 +138,8 @@ struct PagedCfg {
   static constexpr int kOffQ = 2 * kStages * kTileBytes;
   static constexpr int kOffP = kOffQ + kSegs * kQBytes;
   static constexpr int kOffAux = kOffP + 2 * kPBytes;
-  static constexpr int kAux = 384 + 2 * 512 + 192 + kSegs * 16 + 128;
-  static_assert((4 * kStages + 2 * kSegs + 2 * kBufs + 2) * 8 <= 384, "barriers");
+  static constexpr int kAux = 384 + 2 * 512 + 192 + 128 + kSegs * (16 + 128);
+  static_assert((4 * kStages + 2 * kSegs + 2 * kBufs + 3) * 8 <= 384, "barriers");
   static constexpr int kSmem = kOffAux + kAux + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -163,34 +168,62 @@ __device__ void write_empty(const PagedAttnParams& p, int u, int dh) {
   }
 }
 
-__device__ __forceinline__ int share_of(const PagedAttnParams& p, int total) {
-  return max((total + p.grid - 1) / p.grid, p.min_share);
-}
+// How the granules are cut into runs: `grid` of `first` granules (run i belongs to CTA i), the rest in runs of `later`.
+// Beginning a segment costs a CTA about what a tile does, so every unit that holds something counts one tile more
+// (its head): without it a CTA that is given a dozen short sessions ends long after the others.
+struct Cut {
+  int first, later, border, runs;
+  __device__ __forceinline__ Cut(const PagedAttnParams& p, int total) {
+    const int share = max((total + p.grid - 1) / p.grid, p.min_share);
+    first = share;
+    later = 1;
+    // (a run of fewer than 32 tiles ends too soon for the difference to be worth the joins of small ones)
+    if (p.dynamic && share >= 32 * p.min_share) {
+      first = share - 3 * (share >> 4);
+      later = max(share >> 5, 6 * p.min_share);
+    }
+    border = static_cast<int>(min(static_cast<int64_t>(first) * p.grid, static_cast<int64_t>(total)));
+    runs = p.grid + (total - border + later - 1) / later;
+  }
+  __device__ __forceinline__ int run_of(int granule, int grid) const {
+    return granule < border ? granule / first : grid + (granule - border) / later;
+  }
+  __device__ __forceinline__ int64_t begin(int run, int grid) const {
+    return run < grid ? static_cast<int64_t>(run) * first : border + static_cast<int64_t>(run - grid) * later;
+  }
+};
+// Runs there can be at most, per CTA: its own and 3/16 of a share in pieces of 1/32 of it, rounded down to no less than
+// 32 / 33 of that.
+constexpr int kRunsPerCta = 8;
 
-// The pages of a segment's granules, for a warp that loads tiles: 32 granules (four or eight tiles) per look-up of the
+// The pages of a segment's granules, for the warp that loads tiles: 32 granules (four or eight tiles) per look-up of the
 // table, the next 32 under way while these are used.
 struct PageWalk {
   const int32_t* row;        // the session's table row
   int next, end, here, ahead;
 
-  __device__ __forceinline__ int fetch(const PagedAttnParams& p, int lane) {
-    const int tok = next + (lane << p.gran_shift);
-    next += 32 << p.gran_shift;
-    return tok < end ? row[tok >> p.v.page_shift] : 0;
+  // (unchecked: the check waits for the value)
+  __device__ __forceinline__ static int fetch(const PagedAttnParams& p, const int32_t* row, int tok, int end, int lane) {
+    const int t = tok + (lane << p.gran_shift);
+    return t < end ? row[t >> p.v.page_shift] : 0;
   }
-  __device__ __forceinline__ void begin(const PagedAttnParams& p, int s, int tok0, int tok1, int lane) {
+  __device__ __forceinline__ void advance(const PagedAttnParams& p, int lane) {
+    ahead = fetch(p, row, next, end, lane);
+    next += 32 << p.gran_shift;
+  }
+  __device__ __forceinline__ void begin(const PagedAttnParams& p, int s, int tok0, int tok1, int first, int lane) {
     row = p.v.table + s * p.v.table_stride;
-    next = tok0;
+    next = tok0 + (32 << p.gran_shift);
     end = tok1;
-    here = fetch(p, lane);
-    ahead = next < end ? fetch(p, lane) : 0;
+    here = first;
+    advance(p, lane);
   }
   // The page of granule `lane` of the segment's tile `i`.
   __device__ __forceinline__ int page(const PagedAttnParams& p, int i, int lane) {
     const int per = kTile >> p.gran_shift, first = (i * per) & 31;
     if (first == 0 && i > 0) {
       here = ahead;
-      ahead = next < end ? fetch(p, lane) : 0;
+      advance(p, lane);
     }
     int pg = __shfl_sync(0xffffffffu, here, first + (lane & (per - 1)));
     if (pg < 0 || pg >= p.v.n_pages) {
@@ -221,12 +254,15 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   uint64_t* s_full = q_empty + kSegs;
   uint64_t* p_full = s_full + kBufs;
   uint64_t* pv_done = p_full + kBufs;
+  uint64_t* taken = pv_done + 2;
   float* s_max = reinterpret_cast<float*>(aux + 384);                 // [2 groups][4 warps][16]
   float* s_sum = s_max + 128;                                         // [2 groups][4 warps][16]
   float* s_join = s_sum + 128;                                        // group 1's m and l: [2][16]
-  Segment* segs = reinterpret_cast<Segment*>(aux + 1600);
-  int* s_plan = reinterpret_cast<int*>(aux + 1600 + kSegs * 16);      // 0 unit, 1 granule, 2 run, 4.. scan
+  int* s_plan = reinterpret_cast<int*>(aux + 1600);                   // 0 unit, 1 granule, 2 run, 3 held, 4.. scan
+  int* s_pre = s_plan + 16;                                           // [warps] granules before the units of a warp
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_plan + 30);
+  Segment* segs = reinterpret_cast<Segment*>(aux + 1728);
+  int* s_pages = reinterpret_cast<int*>(aux + 1728 + kSegs * 16);     // [segments][32]
   volatile int* s_abort = s_plan + 31;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
@@ -243,7 +279,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     }
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 11);        // eight softmax warps, both issuers, the V producer
+      mbar_init(&q_empty[i], 11);        // eight softmax warps, both issuers, the loader
     }
     for (int i = 0; i < kBufs; ++i) {
       mbar_init(&s_full[i], 1);
@@ -251,6 +287,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     }
     mbar_init(&pv_done[0], 1);
     mbar_init(&pv_done[1], 1);
+    mbar_init(taken, 1);
     *s_abort = 0;
     fence_mbar_init();
   }
@@ -261,7 +298,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   auto held = [&](int u) { return paged_count(p.v, p.lens[u / p.chunks]); };
   const int gs = p.gran_shift;
   auto granules = [&](int n) { return (n + (1 << gs) - 1) >> gs; };
+  auto cost = [&](int n) { return n > 0 ? granules(n) + p.min_share : 0; };
   int end_unit = p.units;
+  const int per = (p.units + kPagedThreads - 1) / kPagedThreads;
+  int total = 0;
   if (p.whole) {
     const int u0 = static_cast<int>(static_cast<int64_t>(p.units) * cta / p.grid);
     end_unit = static_cast<int>(static_cast<int64_t>(p.units) * (cta + 1) / p.grid);
@@ -274,12 +314,11 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     for (int u = u0 + tid; u < end_unit; u += kPagedThreads)
       if (held(u) == 0) write_empty(p, u, DH);
   } else {
-    const int per = (p.units + kPagedThreads - 1) / kPagedThreads;
     const int first = min(tid * per, p.units), last = min(first + per, p.units);
     int sum = 0;
     for (int u = first; u < last; ++u) {
       const int n = held(u);
-      sum += granules(n);
+      sum += cost(n);
       if (n == 0 && u % p.grid == cta) write_empty(p, u, DH);
     }
     int pre = sum;
@@ -289,20 +328,19 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     }
     if (lane == 31) s_plan[4 + warp] = pre;
     __syncthreads();
-    int total = 0;
     for (int w = 0; w < kPagedWarps; ++w) {
       const int y = s_plan[4 + w];
       if (w < warp) pre += y;
       total += y;
     }
     pre -= sum;
-    const int share = share_of(p, total);
-    const int64_t g0 = static_cast<int64_t>(share) * cta;
-    const int run = g0 < total ? static_cast<int>(min(static_cast<int64_t>(share), total - g0)) : 0;
-    if (tid == 0) s_plan[2] = run;
-    if (run > 0 && g0 >= pre && g0 < pre + sum) {
+    if (lane == 0) s_pre[warp] = pre;
+    const Cut cut(p, total);
+    const int64_t g0 = cut.begin(cta, p.grid);
+    if (tid == 0) s_plan[2] = g0 < cut.border ? static_cast<int>(min(static_cast<int64_t>(cut.first), cut.border - g0)) : 0;
+    if (g0 >= pre && g0 < pre + sum) {
       int u = first, at = pre;
-      for (int n = granules(held(u)); at + n <= g0; n = granules(held(++u))) at += n;
+      for (int n = cost(held(u)); at + n <= g0; n = cost(held(++u))) at += n;
       s_plan[0] = u;
       s_plan[1] = static_cast<int>(g0) - at;
       s_plan[3] = held(u);
@@ -311,7 +349,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
       int at = pre;
       for (int u = first; u < last; ++u) {
         p.ws_prefix[u] = at;
-        at += granules(held(u));
+        at += cost(held(u));
       }
       if (tid == 0) p.ws_prefix[p.units] = total;
     }
@@ -322,26 +360,75 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = *s_tmem;
   if (warp == 8) {
-    // ---------------------------------------------------------------- K tiles and segments
-    const uint64_t policy = p.chunks == 1 ? l2_evict_first() : l2_evict_normal();
+    // ---------------------------------------------------------------- segments
     int u = s_plan[0], at = s_plan[1], left = s_plan[2], n = s_plan[3];
-    int seg = 0, it = 0;
+    int seg = 0, run = cta, run_segs = 0;
+    const Cut cut(p, total);
     bool ok = true;
-    while (ok && left > 0 && u < end_unit) {
-      const int n_next = u + 1 < end_unit ? p.lens[(u + 1) / p.chunks] : 0;      // (clamped when its turn comes)
-      const int tok0 = at << gs;
-      int ntok = n - tok0;
-      if (!p.whole) ntok = static_cast<int>(min(static_cast<int64_t>(ntok), static_cast<int64_t>(left) << gs));
-      if (ntok <= 0) {
+    // Takes the next of the runs that are handed out, and finds the unit it starts in.
+    auto take_run = [&]() {
+      int k = 0;
+      if (lane == 0) k = atomicAdd(p.ws_prefix + p.units + 1, 1);
+      run = min(p.grid + __shfl_sync(0xffffffffu, k, 0), cut.runs);
+      run_segs = 0;
+      const int g0 = static_cast<int>(cut.begin(run, p.grid));
+      left = run < cut.runs ? min(cut.later, total - g0) : 0;
+      if (left == 0) return;
+      // as at the set-up each lane takes `per` units of the warp that had the place, then walks its own
+      const uint32_t from = __ballot_sync(0xffffffffu, lane < kPagedWarps && s_pre[lane < kPagedWarps ? lane : 0] <= g0);
+      const int w = 31 - __clz(from), first = min((w * 32 + lane) * per, p.units), last = min(first + per, p.units);
+      int sum = 0;
+      for (int i = first; i < last; ++i) sum += cost(held(i));
+      int upto = sum;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += y;
+      }
+      upto += s_pre[w];
+      const uint32_t hit = __ballot_sync(0xffffffffu, upto > g0);
+      const int l = hit != 0 ? __ffs(hit) - 1 : 0;
+      int i = first, before = upto - sum, mine = 0;
+      for (; i < last; ++i) {
+        mine = held(i);
+        if (before + cost(mine) > g0) break;
+        before += cost(mine);
+      }
+      u = __shfl_sync(0xffffffffu, i, l);
+      n = __shfl_sync(0xffffffffu, mine, l);
+      at = __shfl_sync(0xffffffffu, g0 - before, l);
+      if (hit == 0) left = 0;                              // (the counts changed under us)
+    };
+    while (true) {
+      // one segment ahead of the loader: further ahead, runs would be taken that another CTA could begin sooner
+      if (seg > 0) ok = __all_sync(0xffffffffu, mbar_wait(taken, (seg - 1) & 1, s_abort));
+      if (!ok) break;
+      int n_next = 0, tok0 = 0, ntok = 0;
+      while (true) {
+        if (left <= 0 && cut.runs > p.grid && run < cut.runs) take_run();
+        if (left <= 0 || u >= end_unit) break;
+        n_next = u + 1 < end_unit ? p.lens[(u + 1) / p.chunks] : 0;        // (clamped when its turn comes)
+        const int head = n > 0 ? max(p.min_share - at, 0) : 0;             // of the unit's head, in this run
+        tok0 = max(at - p.min_share, 0) << gs;
+        ntok = n - tok0;
+        if (!p.whole) {
+          ntok = static_cast<int>(min(static_cast<int64_t>(ntok), static_cast<int64_t>(left - head) << gs));
+          left -= head;
+        }
+        if (ntok > 0) break;
         ++u;
         at = 0;
         n = paged_count(p.v, n_next);
-        continue;
+      }
+      const int qslot = seg % kSegs;
+      if (ntok <= 0) {                                     // the end
+        if (mbar_wait(&q_empty[qslot], ((seg / kSegs) & 1) ^ 1, s_abort) && lane == 0) {
+          segs[qslot].ntok = 0;
+          mbar_arrive(&q_full[qslot]);
+        }
+        break;
       }
       const UnitHeads w = unit_heads(p, u);
-      const int qslot = seg % kSegs, end = tok0 + ntok, x0 = w.h * static_cast<int>(p.unit_head);
-      PageWalk walk;
-      walk.begin(p, w.s, tok0, end, lane);
+      const int first_pages = PageWalk::fetch(p, p.v.table + w.s * p.v.table_stride, tok0, tok0 + ntok, lane);
       constexpr int kVecs = DH / 8, kLoads = (GP * kVecs + 31) / 32;
       uint4 q[kLoads];
 #pragma unroll
@@ -352,75 +439,94 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
           q[i] = *reinterpret_cast<const uint4*>(p.q + w.s * p.qs[0] + (w.hq0 + row) * p.qs[1] + 8 * vec);
       }
       ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[qslot], ((seg / kSegs) & 1) ^ 1, s_abort));
-      for (int t0 = tok0; t0 < end && ok; t0 += kTile, ++it) {
-        const int st = it % C::kStages, ng = (min(kTile, end - t0) + (1 << gs) - 1) >> gs;
-        const int pg = walk.page(p, (t0 - tok0) / kTile, lane);
-        ok = mbar_wait(&k_empty[st], ((it / C::kStages) & 1) ^ 1, s_abort);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&k_full[st], (ng << gs) * DH * 2);
-        __syncwarp();
-        if (lane < ng)
-          tma_load_5d(smem_u32(sK + st * C::kTileBytes) + lane * ((DH * 2) << gs), &tm, &k_full[st], 0, 0, 0,
-                      ((t0 + (lane << gs)) & (p.v.page - 1)) >> 3, pg * static_cast<int>(p.unit_page) + x0, policy);
-        if (t0 == tok0) {
-          // the segment's query rows: [chunk][16 rows][128 bytes], 128-byte swizzle
+      if (!ok) break;
+      s_pages[qslot * 32 + lane] = first_pages;
+      // the query rows: [chunk][16 rows][128 bytes], 128-byte swizzle
 #pragma unroll
-          for (int i = 0; i < kLoads; ++i) {
-            const int e = lane + 32 * i, row = e / kVecs, vec = e % kVecs;
-            if (row < GP)
-              *reinterpret_cast<uint4*>(sQ + qslot * C::kQBytes + (vec >> 3) * 2048 + row * 128 +
-                                        (((vec & 7) ^ (row & 7)) << 4)) = q[i];
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            Segment d;
-            d.unit = u;
-            d.tok0 = tok0;
-            d.ntok = ntok;
-            d.slot = (tok0 == 0 && ntok == n) ? -1 : 2 * cta + (seg == 0 ? 0 : 1);
-            segs[qslot] = d;
-            mbar_arrive(&q_full[qslot]);
-          }
-        }
+      for (int i = 0; i < kLoads; ++i) {
+        const int e = lane + 32 * i, row = e / kVecs, vec = e % kVecs;
+        if (row < GP)
+          *reinterpret_cast<uint4*>(sQ + qslot * C::kQBytes + (vec >> 3) * 2048 + row * 128 +
+                                    (((vec & 7) ^ (row & 7)) << 4)) = q[i];
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        Segment d;
+        d.unit = u;
+        d.tok0 = tok0;
+        d.ntok = ntok;
+        d.slot = (tok0 == 0 && ntok == n) ? -1 : 2 * run + (run_segs == 0 ? 0 : 1);
+        segs[qslot] = d;
+        mbar_arrive(&q_full[qslot]);
       }
       ++seg;
+      ++run_segs;
       if (!p.whole) left -= granules(ntok);
       ++u;
       at = 0;
       n = paged_count(p.v, n_next);
     }
-    if (ok && mbar_wait(&q_empty[seg % kSegs], ((seg / kSegs) & 1) ^ 1, s_abort) && lane == 0) {
-      segs[seg % kSegs].ntok = 0;
-      mbar_arrive(&q_full[seg % kSegs]);
-    }
   } else if (warp == 11) {
-    // ---------------------------------------------------------------- V tiles
+    // ---------------------------------------------------------------- K and V tiles
     const uint64_t policy = p.chunks == 1 ? l2_evict_first() : l2_evict_normal();
     int it = 0;
+    // The first segment is plain from the set-up: its first tiles are asked for while warp 8 still gathers its queries.
+    Segment d;
+    d.unit = s_plan[0];
+    d.tok0 = max(s_plan[1] - p.min_share, 0) << gs;
+    d.ntok = s_plan[2] > 0 && d.unit < end_unit ? s_plan[3] - d.tok0 : 0;
+    if (!p.whole && d.ntok > 0)
+      d.ntok = static_cast<int>(min(static_cast<int64_t>(d.ntok),
+                                    static_cast<int64_t>(s_plan[2] - max(p.min_share - s_plan[1], 0)) << gs));
+    bool early = d.ntok > 0;
     for (int seg = 0;; ++seg) {
       const int qslot = seg % kSegs;
-      bool ok = mbar_wait(&q_full[qslot], (seg / kSegs) & 1, s_abort);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      const Segment d = segs[qslot];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_empty[qslot]);
-      if (d.ntok == 0) break;
+      int first_pages = 0;
+      bool ok = true;
+      auto receive = [&]() {                               // the segment as warp 8 published it
+        ok = __all_sync(0xffffffffu, mbar_wait(&q_full[qslot], (seg / kSegs) & 1, s_abort));
+        if (!ok) return;
+        d = segs[qslot];
+        first_pages = s_pages[qslot * 32 + lane];
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&q_empty[qslot]);
+          mbar_arrive(taken);
+        }
+      };
+      if (!early) {
+        receive();
+        if (!ok || d.ntok == 0) break;
+      } else {
+        const int32_t* row = p.v.table + unit_heads(p, d.unit).s * p.v.table_stride;
+        first_pages = PageWalk::fetch(p, row, d.tok0, d.tok0 + d.ntok, lane);
+      }
       const UnitHeads w = unit_heads(p, d.unit);
-      const int end = d.tok0 + d.ntok, x0 = w.h * static_cast<int>(p.unit_head) + static_cast<int>(p.unit_plane);
+      const int end = d.tok0 + d.ntok, x_head = w.h * static_cast<int>(p.unit_head);
       PageWalk walk;
-      walk.begin(p, w.s, d.tok0, end, lane);
+      walk.begin(p, w.s, d.tok0, end, first_pages, lane);
       for (int t0 = d.tok0; t0 < end; t0 += kTile, ++it) {
         const int st = it % C::kStages, ng = (min(kTile, end - t0) + (1 << gs) - 1) >> gs;
         const int pg = walk.page(p, (t0 - d.tok0) / kTile, lane);
-        ok = mbar_wait(&v_empty[st], ((it / C::kStages) & 1) ^ 1, s_abort);
+        const int row = ((t0 + (lane << gs)) & (p.v.page - 1)) >> 3, x = pg * static_cast<int>(p.unit_page) + x_head;
+        const uint32_t at = st * C::kTileBytes + lane * ((DH * 2) << gs), parity = ((it / C::kStages) & 1) ^ 1;
+        ok = mbar_wait(&k_empty[st], parity, s_abort);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (lane == 0) mbar_arrive_expect_tx(&k_full[st], (ng << gs) * DH * 2);
+        __syncwarp();
+        if (lane < ng) tma_load_5d(smem_u32(sK) + at, &tm, &k_full[st], 0, 0, 0, row, x, policy);
+        ok = mbar_wait(&v_empty[st], parity, s_abort);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) mbar_arrive_expect_tx(&v_full[st], (ng << gs) * DH * 2);
         __syncwarp();
         if (lane < ng)
-          tma_load_5d(smem_u32(sV + st * C::kTileBytes) + lane * ((DH * 2) << gs), &tm, &v_full[st], 0, 0, 0,
-                      ((t0 + (lane << gs)) & (p.v.page - 1)) >> 3, pg * static_cast<int>(p.unit_page) + x0, policy);
+          tma_load_5d(smem_u32(sV) + at, &tm, &v_full[st], 0, 0, 0, row, x + static_cast<int>(p.unit_plane), policy);
+        if (early) {
+          early = false;
+          receive();
+          if (!ok) break;
+        }
       }
     }
   } else if (warp == 9) {
@@ -703,18 +809,19 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
 }
 
 // ------------------------------------------------------------------ units that several CTAs share
-// Where the pieces of a unit lie: CTA c0 .. c1, and the workspace slot of each.
+// Where the pieces of a unit lie: in n runs from `run` on, and the workspace slot of each.
 struct Pieces {
-  int c0, n, slot0;
+  int run, n, slot0;
 };
-__device__ __forceinline__ Pieces pieces_of(int a, int b, int share) {
+// (a unit at [a, b) of the granules, its head the first `head` of them)
+__device__ __forceinline__ Pieces pieces_of(const Cut& cut, int a, int b, int head, int grid) {
   Pieces r;
-  r.c0 = a / share;
-  r.n = (b - 1) / share - r.c0 + 1;
-  r.slot0 = 2 * r.c0 + (a == r.c0 * share ? 0 : 1);
+  r.run = cut.run_of(a + head, grid);
+  r.n = cut.run_of(b - 1, grid) - r.run + 1;
+  r.slot0 = 2 * r.run + (cut.begin(r.run, grid) >= a ? 0 : 1);
   return r;
 }
-__device__ __forceinline__ int slot_of_piece(const Pieces& r, int k) { return k == 0 ? r.slot0 : 2 * (r.c0 + k); }
+__device__ __forceinline__ int slot_of_piece(const Pieces& r, int k) { return k == 0 ? r.slot0 : 2 * (r.run + k); }
 
 // Softmax statistics of a head over the pieces of its unit, by one warp: maximum and sum, in every lane.
 template <int GP>
@@ -732,123 +839,150 @@ __device__ __forceinline__ float2 join_ml(const PagedAttnParams& p, const Pieces
 }
 
 template <int DH, bool BF16, int GP>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads, GP >= 8 ? 2 : 3) paged_join_kernel(const PagedAttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kWarps = kJoinThreads / 32, kPer = DH / 32;
   __shared__ float s_o[kWarps][DH];
   __shared__ float s_lse[kMaxGroup];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int total = p.ws_prefix[p.units], share = share_of(p, total);
-  // ---- outputs: one head at a time
-  const int heads = min(p.group, kMaxGroup);
-  for (int64_t item = blockIdx.x; item < static_cast<int64_t>(p.units) * heads; item += gridDim.x) {
-    const int u = static_cast<int>(item / heads), g = static_cast<int>(item - static_cast<int64_t>(u) * heads);
-    const int a = p.ws_prefix[u], b = p.ws_prefix[u + 1];
-    if (a == b) continue;
-    const Pieces r = pieces_of(a, b, share);
-    const UnitHeads w = unit_heads(p, u);
-    if (r.n == 1 || g >= w.n) continue;
-    const float2 ml = join_ml<GP>(p, r, g, lane);
-    float o[kPer];
+  // ---- outputs: a head per block, its pieces dealt out to the warps, or where there are many heads one per warp
+  if (blockIdx.x < p.out_blocks) {
+    const int heads = min(p.group, kMaxGroup);
+    const int64_t items = static_cast<int64_t>(p.units) * heads;
+    const int64_t step = static_cast<int64_t>(p.out_blocks) * (p.out_by_warp ? kWarps : 1);
+    const int first = p.out_by_warp ? 0 : warp, stride = p.out_by_warp ? 1 : kWarps;
+    for (int64_t item = p.out_by_warp ? blockIdx.x * kWarps + warp : blockIdx.x; item < items; item += step) {
+      const int u = static_cast<int>(item / heads), g = static_cast<int>(item - static_cast<int64_t>(u) * heads);
+      const int a = p.ws_prefix[u], b = p.ws_prefix[u + 1], total = p.ws_prefix[p.units];   // (loads that go out together)
+      if (a == b) continue;
+      const Cut cut(p, total);
+      const Pieces r = pieces_of(cut, a, b, p.min_share, p.grid);
+      const UnitHeads w = unit_heads(p, u);
+      if (r.n == 1 || g >= w.n) continue;
+      const float* ws_o = p.ws_o + static_cast<int64_t>(g) * DH + lane;
+      float o[kPer], here[kPer];                           // (the first piece is on its way while the statistics are)
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-    for (int k = warp; k < r.n; k += kWarps) {
-      const int64_t at = static_cast<int64_t>(slot_of_piece(r, k)) * GP + g;
-      const float f = exp2_fast(p.ws_ml[at].x - ml.x);
+      for (int i = 0; i < kPer; ++i) {
+        o[i] = 0.f;
+        here[i] = first < r.n ? ws_o[static_cast<int64_t>(slot_of_piece(r, first)) * GP * DH + 32 * i] : 0.f;
+      }
+      const float2 ml = join_ml<GP>(p, r, g, lane);
+#pragma unroll 2
+      for (int k = first; k < r.n; k += stride) {
+        const float f = exp2_fast(p.ws_ml[slot_of_piece(r, k) * GP + g].x - ml.x);
+        const int next = k + stride;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) o[i] += f * p.ws_o[at * DH + 32 * i + lane];
-    }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) s_o[warp][32 * i + lane] = o[i];
-    __syncthreads();
-    if (tid < DH) {
-      float x = 0.f;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) x += s_o[k][tid];
-      p.out[w.s * p.os[0] + (w.hq0 + g) * p.os[1] + tid] = narrow<BF16>(x / ml.y);
-    }
-    if (tid == 0 && p.lse != nullptr)
-      p.lse[static_cast<int64_t>(w.s) * p.Hq + w.hq0 + g] = (ml.x + log2f(ml.y)) * 0.6931471805599453f;
-    __syncthreads();
-  }
-  if (p.weights == nullptr) return;
-  // ---- weights of the tokens of this CTA's share of the granules; where a kv head has several units, their shares of a
-  // token's weight are added up before they go to memory, in the order of the heads
-  const int gs = p.gran_shift;
-  int at = static_cast<int>(static_cast<int64_t>(total) * blockIdx.x / gridDim.x);
-  const int stop = static_cast<int>(static_cast<int64_t>(total) * (blockIdx.x + 1) / gridDim.x);
-  if (at >= stop) return;
-  __shared__ int s_before[kWarps];                    // units that begin at or before `at`: the last of them holds it
-  int before = 0;
-  for (int u = tid; u < p.units; u += kJoinThreads) before += p.ws_prefix[u] <= at ? 1 : 0;
-  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  if (lane == 0) s_before[warp] = before;
-  __syncthreads();
-  int lo = -1;
-  for (int k = 0; k < kWarps; ++k) lo += s_before[k];
-  for (int u = lo; at < stop; ++u) {
-    const int a = p.ws_prefix[u], b = p.ws_prefix[u + 1];
-    if (a == b) continue;
-    const int from = at - a;
-    at = min(b, stop);
-    if (u % p.chunks != 0) continue;
-    const UnitHeads w = unit_heads(p, u);
-    const int n = min(paged_count(p.v, p.lens[u / p.chunks]), (at - a) << gs);
-    for (int t0 = from << gs; t0 < n; t0 += kJoinThreads * 4) {
-      const int t = t0 + 4 * tid;                       // four neighbours: one page, 16 bytes of each head's logits
-      float add[4] = {0.f, 0.f, 0.f, 0.f};
-      const int pg = t < n ? p.v.table[w.s * p.v.table_stride + (t >> p.v.page_shift)] : 0;
-      for (int c = 0; c < p.chunks; ++c) {
-        const int nh = unit_heads(p, u + c).n;
-        const float* xs = p.ws_x + static_cast<int64_t>(u + c) * GP * p.x_stride + t;
-        float4 x[GP];
-#pragma unroll
-        for (int g = 0; g < GP; ++g)
-          if (t < n && g < nh) x[g] = *reinterpret_cast<const float4*>(xs + g * p.x_stride);
-        if (t0 == from << gs || p.chunks > 1) {
-          const int ca = p.ws_prefix[u + c];
-          const Pieces r = pieces_of(ca, ca + (b - a), share);
-          __syncthreads();
-          for (int g = warp; g < nh; g += kWarps) {
-            float lse;
-            if (r.n == 1) {
-              lse = p.ws_lse[static_cast<int64_t>(u + c) * GP + g];
-            } else {
-              const float2 ml = join_ml<GP>(p, r, g, lane);
-              lse = ml.x + log2f(ml.y);
-            }
-            if (lane == 0) s_lse[g] = lse;
-          }
-          __syncthreads();
-        }
-#pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          if (g >= nh) continue;
-          const float le = s_lse[g];
-          add[0] += exp2_fast(x[g].x - le);
-          add[1] += exp2_fast(x[g].y - le);
-          add[2] += exp2_fast(x[g].z - le);
-          add[3] += exp2_fast(x[g].w - le);
+        for (int i = 0; i < kPer; ++i) {
+          o[i] += f * here[i];
+          here[i] = next < r.n ? ws_o[static_cast<int64_t>(slot_of_piece(r, next)) * GP * DH + 32 * i] : 0.f;
         }
       }
+      uint16_t* out = p.out + w.s * p.os[0] + (w.hq0 + g) * p.os[1];
+      if (p.out_by_warp) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) out[32 * i + lane] = narrow<BF16>(o[i] / ml.y);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) s_o[warp][32 * i + lane] = o[i];
+        __syncthreads();
+        if (tid < DH) {
+          float x = 0.f;
+#pragma unroll
+          for (int k = 0; k < kWarps; ++k) x += s_o[k][tid];
+          out[tid] = narrow<BF16>(x / ml.y);
+        }
+        __syncthreads();
+      }
+      if ((p.out_by_warp ? lane : tid) == 0 && p.lse != nullptr)
+        p.lse[static_cast<int64_t>(w.s) * p.Hq + w.hq0 + g] = (ml.x + log2f(ml.y)) * 0.6931471805599453f;
+    }
+    return;
+  }
+  // ---- weights: `per_item` tokens of a kv head at a time; where it has several units, their shares of a token's weight
+  // are added up before they go to memory, in the order of the heads
+  constexpr int kQuads = GP == 16 ? 1 : 2, kPerItem = kQuads * 4 * kJoinThreads;
+  const int parts = static_cast<int>((p.x_stride + kPerItem - 1) / kPerItem);
+  const int64_t items = static_cast<int64_t>(p.units / p.chunks) * parts;
+  for (int64_t item = blockIdx.x - p.out_blocks; item < items; item += gridDim.x - p.out_blocks) {
+    const int kvh = static_cast<int>(item / parts), t0 = static_cast<int>(item - static_cast<int64_t>(kvh) * parts) * kPerItem;
+    const int total = p.ws_prefix[p.units], held = p.lens[kvh];
+    const int n = paged_count(p.v, held);
+    if (t0 >= n) continue;
+    const Cut cut(p, total);
+    const int s = kvh / p.v.Hkv, h = kvh - s * p.v.Hkv;
+    int pg[kQuads];
+    float add[kQuads][4];
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int t = t0 + 4 * (i * kJoinThreads + tid);    // four neighbours: one page, 16 bytes of each head's logits
+      pg[i] = t < n ? p.v.table[s * p.v.table_stride + (t >> p.v.page_shift)] : 0;
+      add[i][0] = add[i][1] = add[i][2] = add[i][3] = 0.f;
+    }
+    for (int c = 0; c < p.chunks; ++c) {
+      const int u = kvh * p.chunks + c, nh = unit_heads(p, u).n;
+      const float* xs = p.ws_x + static_cast<int64_t>(u) * GP * p.x_stride + t0 + 4 * tid;
+      float4 x[kQuads][GP];
+#pragma unroll
+      for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+        for (int g = 0; g < GP; ++g)
+          if (t0 + 4 * (i * kJoinThreads + tid) < n && g < nh)
+            x[i][g] = *reinterpret_cast<const float4*>(xs + g * p.x_stride + 4 * i * kJoinThreads);
+      const Pieces r = pieces_of(cut, p.ws_prefix[u], p.ws_prefix[u + 1], p.min_share, p.grid);
+      __syncthreads();
+      for (int g = warp; g < nh; g += kWarps) {
+        float lse;
+        if (r.n == 1) {
+          lse = p.ws_lse[static_cast<int64_t>(u) * GP + g];
+        } else {
+          const float2 ml = join_ml<GP>(p, r, g, lane);
+          lse = ml.x + log2f(ml.y);
+        }
+        if (lane == 0) s_lse[g] = lse;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int g = 0; g < GP; ++g) {
+        if (g >= nh) continue;
+        const float le = s_lse[g];
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i) {
+          add[i][0] += exp2_fast(x[i][g].x - le);
+          add[i][1] += exp2_fast(x[i][g].y - le);
+          add[i][2] += exp2_fast(x[i][g].z - le);
+          add[i][3] += exp2_fast(x[i][g].w - le);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int t = t0 + 4 * (i * kJoinThreads + tid);
       if (t >= n) continue;
-      if (pg < 0 || pg >= p.v.n_pages) {
+      if (pg[i] < 0 || pg[i] >= p.v.n_pages) {
         paged_report(p.v);
         continue;
       }
-      float* dst = p.weights + ((static_cast<int64_t>(pg) * p.v.Hkv + w.h) << p.v.page_shift) + (t & (p.v.page - 1));
+      float* dst = p.weights + ((static_cast<int64_t>(pg[i]) * p.v.Hkv + h) << p.v.page_shift) + (t & (p.v.page - 1));
       if (t + 3 < n) {
-        atomicAdd(reinterpret_cast<float4*>(dst), make_float4(add[0], add[1], add[2], add[3]));
+        atomicAdd(reinterpret_cast<float4*>(dst), make_float4(add[i][0], add[i][1], add[i][2], add[i][3]));
       } else {
-        for (int i = 0; t + i < n; ++i) atomicAdd(dst + i, add[i]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          if (t + k < n) atomicAdd(dst + k, add[i][k]);
       }
     }
   }
 }
 
+__global__ void paged_zero_kernel(int32_t* counter) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  *counter = 0;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ------------------------------------------------------------------ host
 struct PagedPlan {
-  int chunks, gp, units, gran_shift, grid, whole, min_share;
+  int chunks, gp, units, gran_shift, grid, whole, min_share, dynamic;
   int64_t cap;
   size_t off_ml, off_o, off_lse, off_x, bytes;
 };
@@ -861,18 +995,22 @@ static int paged_plan(const we_b200_paged_geom& g, int Hq, bool accumulate, Page
   const int64_t units = static_cast<int64_t>(g.S) * g.Hkv * r->chunks;
   r->gran_shift = g.page == 16 ? 4 : 5;
   r->cap = static_cast<int64_t>(g.max_pages) * g.page;
-  const int64_t most = units * (r->cap >> r->gran_shift);           // granules, counted in 32 bits by the kernels
+  r->min_share = kTile >> r->gran_shift;
+  // granules and heads, counted in 32 bits by the kernels
+  const int64_t most = units * ((r->cap >> r->gran_shift) + r->min_share);
   if (units > (1 << 24) || most > 0x3FFFFFFF) return WE_B200_E_LIMIT;
   r->units = static_cast<int>(units);
-  r->min_share = kTile >> r->gran_shift;                            // no less than a tile per CTA
   r->whole = r->cap <= kWholeUnitTokens && !accumulate;
   const int64_t want = r->whole ? units : (most + r->min_share - 1) / r->min_share;
   const int sms = sm_count();
   r->grid = static_cast<int>(want < sms ? want : sms);
+  // (decided by the room the sessions have: what they hold is known on the device only)
+  r->dynamic = !r->whole && r->grid == sms && most / sms >= 32 * r->min_share;
+  const size_t runs = static_cast<size_t>(r->grid) * (r->dynamic ? kRunsPerCta : 1);
   auto up = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
-  r->off_ml = up(sizeof(int32_t) * (r->units + 1));
-  r->off_o = r->off_ml + up(sizeof(float2) * 2 * r->grid * r->gp);
-  r->off_lse = r->off_o + sizeof(float) * 2 * r->grid * r->gp * g.Dh;
+  r->off_ml = up(sizeof(int32_t) * (r->units + 2));
+  r->off_o = r->off_ml + up(sizeof(float2) * 2 * runs * r->gp);
+  r->off_lse = r->off_o + sizeof(float) * 2 * runs * r->gp * g.Dh;
   r->off_x = r->off_lse + up(sizeof(float) * r->units * r->gp);
   r->bytes = r->whole ? 0 : r->off_x;
   if (accumulate) r->bytes += sizeof(float) * static_cast<size_t>(r->units) * r->gp * r->cap;
@@ -914,7 +1052,7 @@ static int paged_map(CUtensorMap* m, const void* kv, const we_b200_paged_geom& g
 }
 
 template <int DH, bool BF16, int GP>
-static int launch_paged(const CUtensorMap& tm, const PagedAttnParams& p, cudaStream_t stream) {
+static int launch_paged(const CUtensorMap& tm, const PagedAttnParams& p, int weight_blocks, cudaStream_t stream) {
   using C = PagedCfg<DH, GP>;
   static std::atomic<bool> done[kMaxDevices];
   int dev = 0;
@@ -939,13 +1077,19 @@ static int launch_paged(const CUtensorMap& tm, const PagedAttnParams& p, cudaStr
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<DH, BF16, GP>, tm, p);
-  g_launches.fetch_add(1, std::memory_order_relaxed);
+  if (p.dynamic) {
+    cudaLaunchConfig_t zero = cfg;
+    zero.gridDim = zero.blockDim = dim3(1, 1, 1);
+    zero.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&zero, paged_zero_kernel, p.ws_prefix + p.units + 1);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+  }
+  if (e == cudaSuccess) {
+    e = cudaLaunchKernelEx(&cfg, paged_attn_kernel<DH, BF16, GP>, tm, p);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+  }
   if (e == cudaSuccess && !p.whole) {
-    // as many CTAs as there can be heads to join or blocks of tokens to give their weights to
-    const int64_t items = static_cast<int64_t>(p.units) * (p.group < kMaxGroup ? p.group : kMaxGroup);
-    const int64_t most = p.weights != nullptr ? 4 * sm_count() : items;
-    cfg.gridDim = dim3(static_cast<unsigned>(most < 4 * sm_count() ? most : 4 * sm_count()), 1, 1);
+    cfg.gridDim = dim3(static_cast<unsigned>(p.out_blocks + weight_blocks), 1, 1);
     cfg.blockDim = dim3(kJoinThreads, 1, 1);
     cfg.dynamicSmemBytes = 0;
     e = cudaLaunchKernelEx(&cfg, paged_join_kernel<DH, BF16, GP>, p);
@@ -957,13 +1101,13 @@ static int launch_paged(const CUtensorMap& tm, const PagedAttnParams& p, cudaStr
 }
 
 template <int DH, bool BF16>
-static int launch_group(int gp, const CUtensorMap& tm, const PagedAttnParams& p, cudaStream_t stream) {
+static int launch_group(int gp, const CUtensorMap& tm, const PagedAttnParams& p, int weight_blocks, cudaStream_t stream) {
   switch (gp) {
-    case 1: return launch_paged<DH, BF16, 1>(tm, p, stream);
-    case 2: return launch_paged<DH, BF16, 2>(tm, p, stream);
-    case 4: return launch_paged<DH, BF16, 4>(tm, p, stream);
-    case 8: return launch_paged<DH, BF16, 8>(tm, p, stream);
-    default: return launch_paged<DH, BF16, 16>(tm, p, stream);
+    case 1: return launch_paged<DH, BF16, 1>(tm, p, weight_blocks, stream);
+    case 2: return launch_paged<DH, BF16, 2>(tm, p, weight_blocks, stream);
+    case 4: return launch_paged<DH, BF16, 4>(tm, p, weight_blocks, stream);
+    case 8: return launch_paged<DH, BF16, 8>(tm, p, weight_blocks, stream);
+    default: return launch_paged<DH, BF16, 16>(tm, p, weight_blocks, stream);
   }
 }
 
@@ -1017,10 +1161,22 @@ extern "C" int we_b200_paged_attn(const we_b200_paged_attn_args* a, int32_t* sta
   p.whole = plan.whole;
   p.min_share = plan.min_share;
   p.scale_log2 = (a->scale > 0.f ? a->scale : 1.0f / sqrtf(static_cast<float>(g.Dh))) * 1.4426950408889634f;
+  p.dynamic = plan.dynamic;
+  // join: a CTA per head to join, or a warp where those would not fit at once, and a CTA per 1024 or 2048 tokens of a kv
+  // head to give them their weights, up to what is resident
+  const int64_t items = static_cast<int64_t>(plan.units) * (p.group < kMaxGroup ? p.group : kMaxGroup);
+  const int sms = sm_count();
+  p.out_by_warp = items > 2 * sms;
+  const int64_t out_blocks = p.out_by_warp ? (items + kJoinThreads / 32 - 1) / (kJoinThreads / 32) : items;
+  p.out_blocks = static_cast<int>(out_blocks < 2 * sms ? out_blocks : (p.out_by_warp ? sms : 2 * sms));
+  const int64_t blocks = static_cast<int64_t>(plan.units) * ((plan.cap + 1023) / 1024);
+  const int weight_blocks = p.weights != nullptr ? static_cast<int>(blocks < 3 * sms ? blocks : 3 * sms) : 0;
   CUtensorMap tm;
   if ((rc = paged_map(&tm, a->kv, g, 1 << plan.gran_shift, &p)) != WE_B200_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (g.Dh == 128)
-    return g.dtype == WE_B200_BF16 ? launch_group<128, true>(plan.gp, tm, p, s) : launch_group<128, false>(plan.gp, tm, p, s);
-  return g.dtype == WE_B200_BF16 ? launch_group<64, true>(plan.gp, tm, p, s) : launch_group<64, false>(plan.gp, tm, p, s);
+    return g.dtype == WE_B200_BF16 ? launch_group<128, true>(plan.gp, tm, p, weight_blocks, s)
+                                   : launch_group<128, false>(plan.gp, tm, p, weight_blocks, s);
+  return g.dtype == WE_B200_BF16 ? launch_group<64, true>(plan.gp, tm, p, weight_blocks, s)
+                                 : launch_group<64, false>(plan.gp, tm, p, weight_blocks, s);
 }
