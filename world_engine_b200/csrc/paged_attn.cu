@@ -48,6 +48,7 @@ constexpr float kFloor = -1.0e38f;         // the reference before the first log
 constexpr int kMaxGroup = 16;              // query heads per unit
 constexpr float kRaise = 8.0f;             // log2 units by which a logit may exceed the reference
 constexpr int kJoinThreads = 256;
+constexpr int kJoinTokens = 4 * kJoinThreads;
 constexpr int kWholeUnitTokens = 128;      // sessions this short are never split
 
 struct PagedAttnParams {
@@ -839,7 +840,7 @@ __device__ __forceinline__ float2 join_ml(const PagedAttnParams& p, const Pieces
 }
 
 template <int DH, bool BF16, int GP>
-__global__ void __launch_bounds__(kJoinThreads, GP >= 8 ? 2 : 3) paged_join_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads, 4) paged_join_kernel(const PagedAttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   constexpr int kWarps = kJoinThreads / 32, kPer = DH / 32;
   __shared__ float s_o[kWarps][DH];
@@ -898,38 +899,43 @@ __global__ void __launch_bounds__(kJoinThreads, GP >= 8 ? 2 : 3) paged_join_kern
     }
     return;
   }
-  // ---- weights: `per_item` tokens of a kv head at a time; where it has several units, their shares of a token's weight
-  // are added up before they go to memory, in the order of the heads
-  constexpr int kQuads = GP == 16 ? 1 : 2, kPerItem = kQuads * 4 * kJoinThreads;
-  const int parts = static_cast<int>((p.x_stride + kPerItem - 1) / kPerItem);
-  const int64_t items = static_cast<int64_t>(p.units / p.chunks) * parts;
+  // ---- weights: 1024 tokens of a kv head at a time, four neighbours per thread (they lie in one page).  The logits come
+  // through shared memory, all heads at once: with loads to registers an SM has half as many bytes on their way.
+  // Where a kv head has several units, their shares of a token's weight are added up before they go to memory, in the
+  // order of the heads.
+  extern __shared__ __align__(128) float s_x[];        // [GP][kJoinTokens]
+  __shared__ uint64_t s_full;
+  __shared__ int s_abort;
+  if (tid == 0) {
+    mbar_init(&s_full, 1);
+    s_abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  uint32_t phase = 0;
+  const int kv_heads = p.units / p.chunks;
+  const int64_t items = static_cast<int64_t>(kv_heads) * ((p.x_stride + kJoinTokens - 1) / kJoinTokens);
   for (int64_t item = blockIdx.x - p.out_blocks; item < items; item += gridDim.x - p.out_blocks) {
-    const int kvh = static_cast<int>(item / parts), t0 = static_cast<int>(item - static_cast<int64_t>(kvh) * parts) * kPerItem;
+    const int part = static_cast<int>(item / kv_heads), kvh = static_cast<int>(item - static_cast<int64_t>(part) * kv_heads);
+    const int t0 = part * kJoinTokens, t = t0 + 4 * tid;
     const int total = p.ws_prefix[p.units], held = p.lens[kvh];
     const int n = paged_count(p.v, held);
     if (t0 >= n) continue;
     const Cut cut(p, total);
     const int s = kvh / p.v.Hkv, h = kvh - s * p.v.Hkv;
-    int pg[kQuads];
-    float add[kQuads][4];
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i) {
-      const int t = t0 + 4 * (i * kJoinThreads + tid);    // four neighbours: one page, 16 bytes of each head's logits
-      pg[i] = t < n ? p.v.table[s * p.v.table_stride + (t >> p.v.page_shift)] : 0;
-      add[i][0] = add[i][1] = add[i][2] = add[i][3] = 0.f;
-    }
+    const int pg = t < n ? p.v.table[s * p.v.table_stride + (t >> p.v.page_shift)] : 0;
+    float add[4] = {0.f, 0.f, 0.f, 0.f};
     for (int c = 0; c < p.chunks; ++c) {
       const int u = kvh * p.chunks + c, nh = unit_heads(p, u).n;
-      const float* xs = p.ws_x + static_cast<int64_t>(u) * GP * p.x_stride + t0 + 4 * tid;
-      float4 x[kQuads][GP];
-#pragma unroll
-      for (int i = 0; i < kQuads; ++i)
-#pragma unroll
-        for (int g = 0; g < GP; ++g)
-          if (t0 + 4 * (i * kJoinThreads + tid) < n && g < nh)
-            x[i][g] = *reinterpret_cast<const float4*>(xs + g * p.x_stride + 4 * i * kJoinThreads);
+      if (warp == 0) {
+        // (whole rows of pages: what lies behind the last token is not used)
+        const uint32_t bytes = static_cast<uint32_t>((min(n - t0, kJoinTokens) + 3) & ~3) * 4;
+        if (lane == 0) mbar_arrive_expect_tx(&s_full, bytes * nh);
+        __syncwarp();
+        if (lane < nh)
+          bulk_load(s_x + lane * kJoinTokens, p.ws_x + (static_cast<int64_t>(u) * GP + lane) * p.x_stride + t0, bytes, &s_full);
+      }
       const Pieces r = pieces_of(cut, p.ws_prefix[u], p.ws_prefix[u + 1], p.min_share, p.grid);
-      __syncthreads();
       for (int g = warp; g < nh; g += kWarps) {
         float lse;
         if (r.n == 1) {
@@ -940,37 +946,39 @@ __global__ void __launch_bounds__(kJoinThreads, GP >= 8 ? 2 : 3) paged_join_kern
         }
         if (lane == 0) s_lse[g] = lse;
       }
+      mbar_wait(&s_full, phase & 1, &s_abort);
+      ++phase;
       __syncthreads();
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-        if (g >= nh) continue;
-        const float le = s_lse[g];
-#pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-          add[i][0] += exp2_fast(x[i][g].x - le);
-          add[i][1] += exp2_fast(x[i][g].y - le);
-          add[i][2] += exp2_fast(x[i][g].z - le);
-          add[i][3] += exp2_fast(x[i][g].w - le);
+      if (t < n) {
+#pragma unroll 4
+        for (int g = 0; g < nh; ++g) {
+          const float4 x = *reinterpret_cast<const float4*>(s_x + g * kJoinTokens + 4 * tid);
+          const float le = s_lse[g];
+          add[0] += exp2_fast(x.x - le);
+          add[1] += exp2_fast(x.y - le);
+          add[2] += exp2_fast(x.z - le);
+          add[3] += exp2_fast(x.w - le);
         }
       }
+      __syncthreads();                                   // before the logits and sums of the next unit
     }
-#pragma unroll
-    for (int i = 0; i < kQuads; ++i) {
-      const int t = t0 + 4 * (i * kJoinThreads + tid);
-      if (t >= n) continue;
-      if (pg[i] < 0 || pg[i] >= p.v.n_pages) {
-        paged_report(p.v);
-        continue;
-      }
-      float* dst = p.weights + ((static_cast<int64_t>(pg[i]) * p.v.Hkv + h) << p.v.page_shift) + (t & (p.v.page - 1));
-      if (t + 3 < n) {
-        atomicAdd(reinterpret_cast<float4*>(dst), make_float4(add[i][0], add[i][1], add[i][2], add[i][3]));
-      } else {
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-          if (t + k < n) atomicAdd(dst + k, add[i][k]);
-      }
+    if (t >= n) continue;
+    if (pg < 0 || pg >= p.v.n_pages) {
+      paged_report(p.v);
+      continue;
     }
+    float* dst = p.weights + ((static_cast<int64_t>(pg) * p.v.Hkv + h) << p.v.page_shift) + (t & (p.v.page - 1));
+    if (t + 3 < n) {
+      atomicAdd(reinterpret_cast<float4*>(dst), make_float4(add[0], add[1], add[2], add[3]));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (t + k < n) atomicAdd(dst + k, add[k]);
+    }
+  }
+  if (s_abort != 0) {
+    if (tid == 0 && p.v.status != nullptr) atomicExch(p.v.status, WE_B200_ST_WAIT_EXPIRED);
+    __nanosleep(1000000);  // let copies that are still in flight land before the CTA goes away
   }
 }
 
@@ -1061,6 +1069,9 @@ static int launch_paged(const CUtensorMap& tm, const PagedAttnParams& p, int wei
   if (dev < 0 || dev >= kMaxDevices) return WE_B200_E_LIMIT;
   if (!done[dev].load(std::memory_order_acquire)) {
     e = cudaFuncSetAttribute(paged_attn_kernel<DH, BF16, GP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(paged_join_kernel<DH, BF16, GP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               GP * kJoinTokens * static_cast<int>(sizeof(float)));
     if (e != cudaSuccess) {
       (void)cudaGetLastError();
       return static_cast<int>(e);
@@ -1091,7 +1102,7 @@ static int launch_paged(const CUtensorMap& tm, const PagedAttnParams& p, int wei
   if (e == cudaSuccess && !p.whole) {
     cfg.gridDim = dim3(static_cast<unsigned>(p.out_blocks + weight_blocks), 1, 1);
     cfg.blockDim = dim3(kJoinThreads, 1, 1);
-    cfg.dynamicSmemBytes = 0;
+    cfg.dynamicSmemBytes = weight_blocks > 0 ? GP * kJoinTokens * sizeof(float) : 0;
     e = cudaLaunchKernelEx(&cfg, paged_join_kernel<DH, BF16, GP>, p);
     g_launches.fetch_add(1, std::memory_order_relaxed);
   }
@@ -1162,15 +1173,15 @@ extern "C" int we_b200_paged_attn(const we_b200_paged_attn_args* a, int32_t* sta
   p.min_share = plan.min_share;
   p.scale_log2 = (a->scale > 0.f ? a->scale : 1.0f / sqrtf(static_cast<float>(g.Dh))) * 1.4426950408889634f;
   p.dynamic = plan.dynamic;
-  // join: a CTA per head to join, or a warp where those would not fit at once, and a CTA per 1024 or 2048 tokens of a kv
-  // head to give them their weights, up to what is resident
+  // join: a CTA per head to join, or a warp where those would not fit at once, and a CTA per 1024 tokens of a kv
+  // head to give them their weights
   const int64_t items = static_cast<int64_t>(plan.units) * (p.group < kMaxGroup ? p.group : kMaxGroup);
   const int sms = sm_count();
   p.out_by_warp = items > 2 * sms;
   const int64_t out_blocks = p.out_by_warp ? (items + kJoinThreads / 32 - 1) / (kJoinThreads / 32) : items;
   p.out_blocks = static_cast<int>(out_blocks < 2 * sms ? out_blocks : (p.out_by_warp ? sms : 2 * sms));
-  const int64_t blocks = static_cast<int64_t>(plan.units) * ((plan.cap + 1023) / 1024);
-  const int weight_blocks = p.weights != nullptr ? static_cast<int>(blocks < 3 * sms ? blocks : 3 * sms) : 0;
+  const int64_t blocks = static_cast<int64_t>(plan.units / plan.chunks) * ((plan.cap + kJoinTokens - 1) / kJoinTokens);
+  const int weight_blocks = p.weights != nullptr ? static_cast<int>(blocks < 16 * sms ? blocks : 16 * sms) : 0;
   CUtensorMap tm;
   if ((rc = paged_map(&tm, a->kv, g, 1 << plan.gran_shift, &p)) != WE_B200_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
