@@ -9,7 +9,6 @@ split-KV workspace and the status word.
 from __future__ import annotations
 
 import ctypes
-import functools
 from typing import Optional, Tuple
 
 import torch
@@ -265,12 +264,13 @@ def block_mask_tables(mask_written: torch.Tensor, tokens_per_frame: int
 # A decoding step makes these calls for every layer, so their cost on the host counts: all checks of shapes, types,
 # strides and devices are one look-up of the values they depend on, and the arguments are packed in one go.
 _status_ptrs = {}
+_append_plans = {}
+_attn_plans = {}
+_MAX_PLANS = 4096
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _meta(t: Optional[torch.Tensor]):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_NONE = (None, None, None, None)
 
 
 def _refuse_grad(*tensors) -> None:
@@ -280,9 +280,10 @@ def _refuse_grad(*tensors) -> None:
 
 
 def _check_paged(kv, table, counts, per_slot, others) -> Tuple[int, ...]:
-    """What every paged entry point checks; the geometry's fields."""
+    """What every paged entry point checks; the geometry's fields.  A tensor is given as its (shape, strides, type,
+    device index), one that is left out as `_NONE`."""
     for meta in (kv, table, *counts, *per_slot, *others):
-        if meta is None:
+        if meta == _NONE:
             continue
         if meta[3] < 0:
             raise RuntimeError("world_engine_b200 runs on CUDA tensors only (sm_100a); there is no CPU path")
@@ -296,10 +297,10 @@ def _check_paged(kv, table, counts, per_slot, others) -> Tuple[int, ...]:
         raise ValueError("table must be int32 [S, max_pages] with contiguous rows")
     S, M = table[0]
     for meta in counts:
-        if meta is not None and (meta[2] != torch.int32 or meta[0] != (S, Hkv) or not _dense(meta)):
+        if meta[2] != torch.int32 or meta[0] != (S, Hkv) or not _dense(meta):
             raise ValueError("token counts and positions must be contiguous int32 [S, Hkv]")
     for meta, want in zip(per_slot, (torch.float32, torch.int32)):
-        if meta is not None and (meta[2] != want or meta[0] != (P, Hkv, page) or not _dense(meta)):
+        if meta != _NONE and (meta[2] != want or meta[0] != (P, Hkv, page) or not _dense(meta)):
             raise ValueError("weights (float32) and positions (int32) must be contiguous [pages, Hkv, page]")
     return (S, Hkv, Dh, page, P, M, dtype_code(dtype), 0, stride[0], stride[1], stride[2], stride[3], table[1][0])
 
@@ -318,7 +319,7 @@ def _call_paged(fn, args: bytes, index: int, where: str) -> None:
     status = _status_ptrs.get(index)
     if status is None:
         status = _status_ptrs[index] = status_word(torch.device("cuda", index)).data_ptr()
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         rc = fn(args, status, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -327,9 +328,16 @@ def _call_paged(fn, args: bytes, index: int, where: str) -> None:
         _lib.check(rc, where)
 
 
-@functools.lru_cache(maxsize=1024)
+def _plan(plans, make, key):
+    """The plan of a call nobody made before (a plan depends on nothing but the values in its key)."""
+    if len(plans) >= _MAX_PLANS:
+        plans.clear()
+    plans[key] = plan = make(*(key[i:i + 4] for i in range(0, len(key) // 4 * 4, 4)), *key[len(key) // 4 * 4:])
+    return plan
+
+
 def _append_plan(kv, table, lens, next_pos, lens_out, next_pos_out, k_new, v_new, n_new, weights, positions, w_new,
-                 keep):
+                 keep=0):
     """Checks of an append; (geometry, strides of k_new and v_new, strides of w_new, T, workspace bytes)."""
     geom = _check_paged(kv, table, (lens, next_pos, lens_out, next_pos_out), (weights, positions),
                         (k_new, v_new, n_new, w_new))
@@ -338,14 +346,14 @@ def _append_plan(kv, table, lens, next_pos, lens_out, next_pos_out, k_new, v_new
     if len(shape) != 4 or (shape[0], shape[1], shape[3]) != (S, Hkv, Dh) or v_new[0] != shape \
             or k_new[2] != kv[2] or v_new[2] != kv[2] or k_new[1][3] != 1 or v_new[1][3] != 1:
         raise ValueError("k_new and v_new must be [S, Hkv, T, Dh] of the cache's type with a contiguous last axis")
-    if n_new is not None and (n_new[2] != torch.int32 or n_new[0] != (S,) or not _dense(n_new)):
+    if n_new != _NONE and (n_new[2] != torch.int32 or n_new[0] != (S,) or not _dense(n_new)):
         raise ValueError("n_new must be contiguous int32 [S]")
-    if w_new is not None and (w_new[2] != torch.float32 or w_new[0] != shape[:3]):
+    if w_new != _NONE and (w_new[2] != torch.float32 or w_new[0] != shape[:3]):
         raise ValueError("w_new must be float32 [S, Hkv, T]")
     need = 0
     if keep > 0:
         need = _lib.load().we_b200_paged_evict_workspace_bytes(ctypes.byref(PagedGeom(*geom)), shape[2], keep)
-    return geom, (*k_new[1][:3], *v_new[1][:3]), w_new[1] if w_new is not None else (0, 0, 0), shape[2], need
+    return geom, (*k_new[1][:3], *v_new[1][:3]), w_new[1] if w_new != _NONE else (0, 0, 0), shape[2], need
 
 
 def _append(fn, where, kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new, lens_out,
@@ -354,16 +362,28 @@ def _append(fn, where, kv, table, lens, next_pos, k_new, v_new, n_new, weights, 
     next_pos_out = next_pos if next_pos_out is None else next_pos_out
     if torch.is_grad_enabled():
         _refuse_grad(kv, k_new, v_new, weights, w_new)
-    geom, strides, w_strides, T, need = _append_plan(
-        _meta(kv), _meta(table), _meta(lens), _meta(next_pos), _meta(lens_out), _meta(next_pos_out), _meta(k_new),
-        _meta(v_new), _meta(n_new), _meta(weights), _meta(positions), _meta(w_new), keep)
+    index = kv.get_device()
+    key = (kv.shape, kv.stride(), kv.dtype, index,
+           table.shape, table.stride(), table.dtype, table.get_device(),
+           lens.shape, lens.stride(), lens.dtype, lens.get_device(),
+           next_pos.shape, next_pos.stride(), next_pos.dtype, next_pos.get_device(),
+           lens_out.shape, lens_out.stride(), lens_out.dtype, lens_out.get_device(),
+           next_pos_out.shape, next_pos_out.stride(), next_pos_out.dtype, next_pos_out.get_device(),
+           k_new.shape, k_new.stride(), k_new.dtype, k_new.get_device(),
+           v_new.shape, v_new.stride(), v_new.dtype, v_new.get_device(),
+           *(_NONE if n_new is None else (n_new.shape, n_new.stride(), n_new.dtype, n_new.get_device())),
+           *(_NONE if weights is None else (weights.shape, weights.stride(), weights.dtype, weights.get_device())),
+           *(_NONE if positions is None else
+             (positions.shape, positions.stride(), positions.dtype, positions.get_device())),
+           *(_NONE if w_new is None else (w_new.shape, w_new.stride(), w_new.dtype, w_new.get_device())), keep)
+    geom, strides, w_strides, T, need = _append_plans.get(key) or _plan(_append_plans, _append_plan, key)
     ws = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
     _call_paged(fn, _lib.PAGED_APPEND_PACK.pack(
         *geom, k_new.data_ptr(), v_new.data_ptr(), *strides, kv.data_ptr(),
         0 if weights is None else weights.data_ptr(), 0 if positions is None else positions.data_ptr(),
         table.data_ptr(), lens.data_ptr(), next_pos.data_ptr(), lens_out.data_ptr(), next_pos_out.data_ptr(),
         0 if n_new is None else n_new.data_ptr(), 0 if w_new is None else w_new.data_ptr(), *w_strides,
-        0 if ws is None else ws.data_ptr(), need, T, keep, sink, recent), kv.get_device(), where)
+        0 if ws is None else ws.data_ptr(), need, T, keep, sink, recent), index, where)
 
 
 def paged_append_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, next_pos: torch.Tensor,
@@ -397,7 +417,6 @@ def paged_append_evict_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tenso
             v_new, n_new, weights, positions, w_new, lens_out, next_pos_out, keep, sink, recent)
 
 
-@functools.lru_cache(maxsize=1024)
 def _attn_plan(q, kv, table, lens, weights, out, lse):
     """Checks of an attention call; (geometry, workspace bytes)."""
     geom = _check_paged(kv, table, (lens,), (weights,), (q, out, lse))
@@ -405,12 +424,12 @@ def _attn_plan(q, kv, table, lens, weights, out, lse):
     shape = q[0]
     if len(shape) != 4 or (shape[0], shape[2], shape[3]) != (S, 1, Dh) or q[2] != kv[2] or q[1][3] != 1:
         raise ValueError("q must be [S, Hq, 1, Dh] of the cache's type with a contiguous last axis")
-    if out is not None and (out[0] != shape or out[2] != q[2] or out[1][3] != 1):
+    if out != _NONE and (out[0] != shape or out[2] != q[2] or out[1][3] != 1):
         raise ValueError("out must have q's shape and type and a contiguous last axis")
-    if lse is not None and (lse[2] != torch.float32 or lse[0] != shape[:2] or not _dense(lse)):
+    if lse != _NONE and (lse[2] != torch.float32 or lse[0] != shape[:2] or not _dense(lse)):
         raise ValueError("lse must be contiguous float32 [S, Hq]")
-    need = _lib.load().we_b200_paged_attn_workspace_bytes(ctypes.byref(PagedGeom(*geom)), shape[1], weights is not None)
-    return geom, need
+    need = _lib.load().we_b200_paged_attn_workspace_bytes(ctypes.byref(PagedGeom(*geom)), shape[1], weights != _NONE)
+    return geom, (S, shape[1], 1, Dh), need
 
 
 def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float = 0.0,
@@ -422,16 +441,23 @@ def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: tor
     receives the logarithm of the softmax sum.  A kv head that holds nothing gives 0 and -inf."""
     if torch.is_grad_enabled():
         _refuse_grad(q, kv, weights, out, lse)
-    geom, need = _attn_plan(_meta(q), _meta(kv), _meta(table), _meta(lens), _meta(weights), _meta(out), _meta(lse))
-    Hq = q.shape[1]
+    index, qs = q.get_device(), q.stride()
+    key = (q.shape, qs, q.dtype, index,
+           kv.shape, kv.stride(), kv.dtype, kv.get_device(),
+           table.shape, table.stride(), table.dtype, table.get_device(),
+           lens.shape, lens.stride(), lens.dtype, lens.get_device(),
+           *(_NONE if weights is None else (weights.shape, weights.stride(), weights.dtype, weights.get_device())),
+           *(_NONE if out is None else (out.shape, out.stride(), out.dtype, out.get_device())),
+           *(_NONE if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.get_device())))
+    geom, shape, need = _attn_plans.get(key) or _plan(_attn_plans, _attn_plan, key)
     if out is None:
-        out = q.new_empty((geom[0], Hq, 1, geom[2]))
+        out = q.new_empty(shape)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    qs, os_ = q.stride(), out.stride()
+    os_ = out.stride()
     _call_paged(_lib.load().we_b200_paged_attn, _lib.PAGED_ATTN_PACK.pack(
         *geom, q.data_ptr(), out.data_ptr(), qs[0], qs[1], os_[0], os_[1], kv.data_ptr(), table.data_ptr(),
         lens.data_ptr(), 0 if weights is None else weights.data_ptr(), 0 if lse is None else lse.data_ptr(),
-        0 if ws is None else ws.data_ptr(), need, Hq, scale), q.get_device(), "we_b200_paged_attn")
+        0 if ws is None else ws.data_ptr(), need, shape[1], scale), index, "we_b200_paged_attn")
     return out
 
 
