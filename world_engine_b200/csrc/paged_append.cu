@@ -7,8 +7,8 @@
 // Under a budget the cluster first finds the key of the last token to keep: weights are mapped to unsigned numbers of
 // the same order (shielded tokens above all) and the keep-th largest is found digit by digit, each CTA counting
 // the digits of its slice of the candidates and adding up the other CTAs' counts through cluster shared memory.  One
-// pass over weights and positions in global memory; the later passes read keys from shared memory (slices that do not
-// fit are recomputed from global memory).  Then each CTA lists, in the order of the indexes, the holes of its slice
+// pass over weights and positions in global memory: the keys stay in registers (those of longer slices are read again
+// for every digit).  Then each CTA lists, in the order of the indexes, the holes of its slice
 // (indexes below the budget that are given up) and the movers (kept ones behind it), and the j-th mover goes to the
 // j-th hole: as many rows are copied as tokens leave, not as many as stay.
 #include "paged.cuh"
@@ -167,45 +167,58 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// Three digits of 11, 11 and 10 bits.  (Of 8 bits there are four: with the cluster's barrier and the search in every
-// pass that took 1 to 2 us more per call; most weights differ within the first two digits of 11.)
-constexpr int kPasses = 3, kBins = 2048;
-__host__ __device__ constexpr int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
-__host__ __device__ constexpr uint32_t digit_mask(int pass) { return pass == 2 ? 1023u : 2047u; }
+// In one CTA: three digits of 11, 11 and 10 bits.  In a cluster four of 8: every CTA reads the counts of all others
+// through cluster shared memory, and with 2048 of them that took 3 to 5 us a digit (65536 candidates in eight CTAs).
+constexpr int kHistWords = 3 * 2048;
+struct Digits {
+  int bits, passes;
+  __device__ __forceinline__ explicit Digits(int cluster) : bits(cluster == 1 ? 11 : 8), passes(cluster == 1 ? 3 : 4) {}
+  __device__ __forceinline__ int shift(int pass) const { return max(32 - bits * (pass + 1), 0); }
+  __device__ __forceinline__ uint32_t mask(int pass) const { return (1u << min(bits, 32 - bits * pass)) - 1u; }
+};
 
 // Sum of x over the threads before this one; *all gets the sum over the block.  (One copy for all its uses: a call of
 // this kernel is a few microseconds, and fetching code that runs once is a part of that.)
-template <int kThreads>
-__device__ __noinline__ uint64_t block_scan(uint64_t x, uint64_t* s_warp, uint64_t* all) {
+template <int kThreads, class T>
+__device__ __noinline__ T block_scan(T x, uint64_t* s_warp, T* all) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  uint64_t upto = x;
+  T upto = x;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const uint64_t y = __shfl_up_sync(0xffffffffu, upto, d);
+    const T y = __shfl_up_sync(0xffffffffu, upto, d);
     if (lane >= d) upto += y;
   }
   __syncthreads();                                       // (s_warp may still be read from the call before)
   if (lane == 31) s_warp[wid] = upto;
   __syncthreads();
-  uint64_t w = lane < kWarps ? s_warp[lane] : 0;
+  T w = lane < kWarps ? static_cast<T>(s_warp[lane]) : 0;
+  if constexpr (sizeof(T) == 4) {
+    *all = __reduce_add_sync(0xffffffffu, w);
+    return upto - x + __reduce_add_sync(0xffffffffu, lane < wid ? w : 0);
+  } else {
 #pragma unroll
-  for (int d = 1; d < kWarps; d <<= 1) {
-    const uint64_t y = __shfl_up_sync(0xffffffffu, w, d);
-    if (lane >= d) w += y;
+    for (int d = 1; d < kWarps; d <<= 1) {
+      const T y = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w += y;
+    }
+    *all = __shfl_sync(0xffffffffu, w, kWarps - 1);
+    const T before = __shfl_sync(0xffffffffu, w, wid > 0 ? wid - 1 : 0);
+    return upto - x + (wid > 0 ? before : 0);
   }
-  *all = __shfl_sync(0xffffffffu, w, kWarps - 1);
-  const uint64_t before = __shfl_sync(0xffffffffu, w, wid > 0 ? wid - 1 : 0);
-  return upto - x + (wid > 0 ? before : 0);
 }
 
+// Candidates a thread holds in registers: five times four neighbours.  A slice of up to kThreads * 20 is read once;
+// a longer one (a session that held much more than its budget) is read again for every pass, a round at a time.
+constexpr int kGroups = 5;
+
 template <int kThreads>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) paged_append_evict_kernel(const PagedAppendParams p) {
-  constexpr int kWarps = kThreads / 32, kOwn = kBins / kThreads;
+__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) paged_append_evict_kernel(const PagedAppendParams p) {
+  constexpr int kRound = kThreads * 4 * kGroups, kBatch = kThreads == 256 ? 2 : 3;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  extern __shared__ __align__(16) uint32_t s_keys[];   // [fit] keys, holes, movers, [fit / 32] twice: bits
-  __shared__ __align__(16) uint32_t s_hist[kPasses][kBins];
+  extern __shared__ __align__(16) int32_t s_lists_mem[];  // holes [fit], movers [fit], bits [fit / 32] twice
+  __shared__ __align__(16) uint32_t s_hist[kHistWords];
   __shared__ uint64_t s_warp[32];
   __shared__ uint32_t s_found[3];                      // digit, how many of it are kept, how many there are
   __shared__ int s_equal, s_lists[3];                  // of this CTA: equal keys; holes, movers, new ones in place
@@ -213,7 +226,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) paged_append_evict_
   const int unit = blockIdx.x / p.cluster, rank = blockIdx.x - unit * p.cluster;
   const int s = unit / p.v.Hkv, h = unit - s * p.v.Hkv;
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  for (int b = tid; b < kPasses * kBins / 4; b += kThreads) reinterpret_cast<uint4*>(s_hist)[b] = make_uint4(0u, 0u, 0u, 0u);
+  const Digits digits(p.cluster);
+  const int bins = 1 << digits.bits;
+  for (int b = tid; b < digits.passes * bins / 4; b += kThreads) reinterpret_cast<uint4*>(s_hist)[b] = make_uint4(0u, 0u, 0u, 0u);
   const int len = paged_count(p.v, p.lens[unit]);
   const int pos0 = p.next_pos[unit];
   const int n = new_count(p, s);
@@ -224,111 +239,105 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) paged_append_evict_
     move_tokens<2>(p, s, h, len, pos0, n, rank * kThreads + tid, p.cluster * kThreads,
                    [&](int e, int* src, int* dst) { *src = *dst = len + e; });
   } else {
-    // ---- keys of this CTA's slice, four neighbours at a time (they lie in one page), with the first digit's counts
+    // ---- this CTA's slice of the candidates, in rounds; a thread has four neighbours at a time (they lie in one page)
     const int slice = ((total + p.cluster - 1) / p.cluster + 3) & ~3;
     const int lo = min(rank * slice, total), hi = min(lo + slice, total), mine = hi - lo;
+    const int rounds = (mine + kRound - 1) / kRound;
     const bool fits = slice <= p.fit;
     auto key_of = [&](float w, int64_t pos) {
       return pos < p.sink || pos >= end - p.recent ? 0xFFFFFFFFu : weight_key(w);
     };
-    auto key_at = [&](int i) -> uint32_t {              // one candidate, from global memory
-      if (i >= len) return key_of(new_weight(p, s, h, i - len), static_cast<int64_t>(pos0) + (i - len));
-      const int pg = paged_page(p.v, s, i >> p.v.page_shift);
-      if (pg < 0) return 0u;
-      const int64_t m = meta_index(p, pg, h, i & (p.v.page - 1));
-      return key_of(p.weights[m], p.positions[m]);
-    };
-    // four neighbours from index i on (lo + a multiple of 4); those behind the slice read as 0
-    auto keys4 = [&](int i) -> uint4 {
-      if (fits) return *reinterpret_cast<const uint4*>(s_keys + (i - lo));
-      uint4 k;
-      k.x = i < hi ? key_at(i) : 0u;
-      k.y = i + 1 < hi ? key_at(i + 1) : 0u;
-      k.z = i + 2 < hi ? key_at(i + 2) : 0u;
-      k.w = i + 3 < hi ? key_at(i + 3) : 0u;
-      return k;
-    };
-    constexpr int kDepth = 2;
-    for (int i0 = lo + 4 * tid; i0 < hi; i0 += 4 * kThreads * kDepth) {
-      int pg[kDepth];
-      float4 w[kDepth];
-      int4 pos[kDepth];
+    uint32_t key[kGroups][4];                            // (those behind the slice: unused)
+    auto first_of = [&](int round, int g) { return lo + round * kRound + 4 * (g * kThreads + tid); };
+    auto load = [&](int round) {
+      int pg[kGroups];
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        const int i = i0 + 4 * kThreads * d;
-        pg[d] = i < hi && i + 3 < len ? p.v.table[s * p.v.table_stride + (i >> p.v.page_shift)] : -1;
+      for (int g = 0; g < kGroups; ++g) {
+        const int i = first_of(round, g);
+        pg[g] = i < hi && i < len ? p.v.table[s * p.v.table_stride + (i >> p.v.page_shift)] : 0;
       }
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        if (pg[d] < 0 || pg[d] >= p.v.n_pages) continue;
-        const int64_t m = meta_index(p, pg[d], h, (i0 + 4 * kThreads * d) & (p.v.page - 1));
-        w[d] = *reinterpret_cast<const float4*>(p.weights + m);
-        pos[d] = *reinterpret_cast<const int4*>(p.positions + m);
-      }
+      for (int g0 = 0; g0 < kGroups; g0 += kBatch) {
+        float4 w[kBatch];
+        int4 pos[kBatch];
 #pragma unroll
-      for (int d = 0; d < kDepth; ++d) {
-        const int i = i0 + 4 * kThreads * d;
-        if (i >= hi) continue;
-        uint32_t k[4];
-        if (pg[d] >= 0 && pg[d] < p.v.n_pages) {
-          k[0] = key_of(w[d].x, pos[d].x);
-          k[1] = key_of(w[d].y, pos[d].y);
-          k[2] = key_of(w[d].z, pos[d].z);
-          k[3] = key_of(w[d].w, pos[d].w);
-        } else {                                        // new tokens, the last held ones, a bad page (reported)
-#pragma unroll
-          for (int u = 0; u < 4; ++u) k[u] = i + u < hi ? key_at(i + u) : 0u;
+        for (int b = 0; b < kBatch && g0 + b < kGroups; ++b) {
+          const int g = g0 + b, i = first_of(round, g);
+          w[b] = make_float4(0.f, 0.f, 0.f, 0.f);
+          pos[b] = make_int4(0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF);
+          if (i >= hi || i >= len) continue;
+          if (pg[g] < 0 || pg[g] >= p.v.n_pages) {       // taken for tokens nobody looked at
+            paged_report(p.v);
+            continue;
+          }
+          const int64_t m = meta_index(p, pg[g], h, i & (p.v.page - 1));
+          w[b] = *reinterpret_cast<const float4*>(p.weights + m);
+          pos[b] = *reinterpret_cast<const int4*>(p.positions + m);
         }
-        if (fits) *reinterpret_cast<uint4*>(s_keys + (i - lo)) = make_uint4(k[0], k[1], k[2], k[3]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (i + u < hi) atomicAdd(&s_hist[0][k[u] >> digit_shift(0)], 1u);
+        for (int b = 0; b < kBatch && g0 + b < kGroups; ++b) {
+          const int g = g0 + b, i = first_of(round, g);
+          if (i >= hi) continue;
+          key[g][0] = key_of(w[b].x, pos[b].x);
+          key[g][1] = key_of(w[b].y, pos[b].y);
+          key[g][2] = key_of(w[b].z, pos[b].z);
+          key[g][3] = key_of(w[b].w, pos[b].w);
+          if (i + 3 < len) continue;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (i + u >= len)
+              key[g][u] = i + u < hi ? key_of(new_weight(p, s, h, i + u - len), static_cast<int64_t>(pos0) + (i + u - len)) : 0u;
+        }
       }
-    }
+    };
+    if (rounds == 1) load(0);
     // ---- the key of the last one kept (its leading digits, as far as they decide), how many of that key are kept
     uint32_t prefix = 0, mask = 0, need = static_cast<uint32_t>(p.keep), equals = 0;
 #pragma unroll 1
-    for (int pass = 0; pass < kPasses; ++pass) {
-      const int shift = digit_shift(pass);
-      const uint32_t bits = digit_mask(pass);
-      if (pass > 0) {
-        for (int i = lo + 4 * tid; i < hi; i += 4 * kThreads) {
-          const uint4 k4 = keys4(i);
-          const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+    for (int pass = 0; pass < digits.passes; ++pass) {
+      const int shift = digits.shift(pass);
+      const uint32_t low = digits.mask(pass);
+      uint32_t* hist = s_hist + pass * bins;
+      for (int round = 0; round < rounds; ++round) {
+        if (rounds > 1) load(round);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const int i = first_of(round, g);
+          if (i >= hi) continue;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            if (i + u < hi && (k[u] & mask) == prefix) atomicAdd(&s_hist[pass][(k[u] >> shift) & bits], 1u);
+            if (i + u < hi && (key[g][u] & mask) == prefix) atomicAdd(&hist[(key[g][u] >> shift) & low], 1u);
         }
       }
       unit_sync(p);
-      // kOwn bins per thread, the largest digits in thread 0; a scan over the block finds the one with the keep-th
+      // the largest digits to thread 0; a scan over the block finds the one with the keep-th
+      constexpr int kOwn = 2048 / kThreads;
       uint32_t c[kOwn], sum = 0;
-      const int bin0 = kBins - kOwn * (tid + 1);
+      int bin0 = 0;
+      if (p.cluster == 1) {
+        bin0 = 2048 - kOwn * (tid + 1);
 #pragma unroll
-      for (int b = 0; b < kOwn; ++b) c[b] = 0;
+        for (int b = 0; b < kOwn; b += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(hist + bin0 + b);
+          c[b] = x.x;
+          c[b + 1] = x.y;
+          c[b + 2] = x.z;
+          c[b + 3] = x.w;
+        }
+      } else {
 #pragma unroll
-      for (int r = 0; r < kMaxCluster; ++r) {
-        if (r >= p.cluster) break;
-        const uint32_t* from = p.cluster == 1 ? &s_hist[pass][bin0] : of_rank(&s_hist[pass][bin0], r);
-        if constexpr (kOwn == 2) {
-          const uint2 x = *reinterpret_cast<const uint2*>(from);
-          c[0] += x.x;
-          c[1] += x.y;
-        } else {
+        for (int b = 0; b < kOwn; ++b) c[b] = 0;
+        if (tid < 256) {
+          bin0 = 255 - tid;
 #pragma unroll
-          for (int b = 0; b < kOwn; b += 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(from + b);
-            c[b] += x.x;
-            c[b + 1] += x.y;
-            c[b + 2] += x.z;
-            c[b + 3] += x.w;
-          }
+          for (int r = 0; r < kMaxCluster; ++r)
+            if (r < p.cluster) c[0] += *of_rank(hist + bin0, r);
         }
       }
 #pragma unroll
       for (int b = 0; b < kOwn; ++b) sum += c[b];
-      uint64_t all;
-      const uint32_t before = static_cast<uint32_t>(block_scan<kThreads>(sum, s_warp, &all));
+      uint32_t all;
+      const uint32_t before = block_scan<kThreads, uint32_t>(sum, s_warp, &all);
       if (before < need && before + sum >= need) {
         uint32_t at = before;
         bool found = false;
@@ -345,39 +354,56 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) paged_append_evict_
       }
       __syncthreads();
       prefix |= s_found[0] << shift;
-      mask |= bits << shift;
+      mask |= low << shift;
       need = s_found[1];
       equals = s_found[2];
       if (equals == need) break;                         // everything with these digits stays
     }
     // ---- one bit per candidate: kept outright, or one of the equal keys of which only some are kept
-    int32_t* holes = fits ? reinterpret_cast<int32_t*>(s_keys) + p.fit : p.ws + blockIdx.x * p.ws_chunk;
+    int32_t* holes = fits ? s_lists_mem : p.ws + blockIdx.x * p.ws_chunk;
     const int64_t room = fits ? p.fit : p.ws_stride;
     int32_t* movers = holes + room;
     uint32_t* bits_kept = reinterpret_cast<uint32_t*>(movers + room);
     uint32_t* bits_equal = bits_kept + ((room + 31) >> 5);
     const bool ties = equals != need;
     const int words = (mine + 31) >> 5;
-#pragma unroll 2
-    for (int w = wid; w < words; w += kWarps) {
-      const int i = lo + 32 * w + lane;
-      const uint32_t k = i < hi ? (fits ? s_keys[i - lo] : key_at(i)) & mask : 0u;
-      const uint32_t more = __ballot_sync(0xffffffffu, i < hi && k > prefix);
-      const uint32_t same = __ballot_sync(0xffffffffu, i < hi && k == prefix);
-      if (lane == 0) {
-        bits_kept[w] = ties ? more : more | same;
-        bits_equal[w] = same;
+    for (int round = 0; round < rounds; ++round) {
+      if (rounds > 1) load(round);
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int i = first_of(round, g);
+        if (i - 4 * lane >= hi) continue;                // (the same for the whole warp)
+        uint32_t more = 0, same = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t k = key[g][u] & mask;
+          more |= i + u < hi && k > prefix ? 1u << u : 0u;
+          same |= i + u < hi && k == prefix ? 1u << u : 0u;
+        }
+        if (!ties) more |= same;
+        const int at = 4 * (lane & 7);                   // eight lanes make a word
+        more <<= at;
+        same <<= at;
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) {
+          more |= __shfl_xor_sync(0xffffffffu, more, d);
+          same |= __shfl_xor_sync(0xffffffffu, same, d);
+        }
+        const int w = (i - lo) >> 5;
+        if ((lane & 7) == 0 && w < words) {
+          bits_kept[w] = more;
+          bits_equal[w] = same;
+        }
       }
     }
     __syncthreads();
     // a thread goes on with `per` neighbouring words
     const int per = (words + kThreads - 1) / kThreads, w0 = min(tid * per, words), w1 = min(w0 + per, words);
     if (ties) {                                          // the first `need` of them, in the order of the indexes
-      uint32_t cnt = 0;
+      uint32_t cnt = 0, all;
       for (int w = w0; w < w1; ++w) cnt += __popc(bits_equal[w]);
-      uint64_t all;
       int64_t left = need;
-      left -= static_cast<int64_t>(block_scan<kThreads>(cnt, s_warp, &all));
+      left -= block_scan<kThreads, uint32_t>(cnt, s_warp, &all);
       if (p.cluster > 1) {
         if (tid == 0) s_equal = static_cast<int>(all);
         unit_sync(p);
@@ -399,27 +425,26 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) paged_append_evict_
     };
     auto split = [&](int w, uint32_t* hole, uint32_t* mover, uint32_t* stay) {
       const int base = lo + 32 * w;
-      const uint32_t kept = bits_kept[w], in = ~bits_from(base, hi), beyond = bits_from(base, p.keep);
-      *hole = ~kept & in & ~beyond;
+      const uint32_t kept = bits_kept[w], beyond = bits_from(base, p.keep);
+      *hole = ~kept & ~bits_from(base, hi) & ~beyond;
       *mover = kept & beyond;
       *stay = kept & ~beyond & bits_from(base, len);
     };
-    uint64_t sums = 0;                                   // 21 bits each
+    uint64_t sums = 0, all;                              // 21 bits each
     for (int w = w0; w < w1; ++w) {
       uint32_t b[3];
       split(w, &b[0], &b[1], &b[2]);
       sums += static_cast<uint64_t>(__popc(b[0])) | (static_cast<uint64_t>(__popc(b[1])) << 21) |
               (static_cast<uint64_t>(__popc(b[2])) << 42);
     }
-    uint64_t all;
-    const uint64_t at = block_scan<kThreads>(sums, s_warp, &all);
+    const uint64_t at = block_scan<kThreads, uint64_t>(sums, s_warp, &all);
     int64_t at_h = at & 0x1FFFFF, at_m = (at >> 21) & 0x1FFFFF, at_s = at >> 42;
     if (tid == 0) {
       s_lists[0] = static_cast<int>(all & 0x1FFFFF);
       s_lists[1] = static_cast<int>((all >> 21) & 0x1FFFFF);
       s_lists[2] = static_cast<int>(all >> 42);
     }
-    for (int w = w0; w < w1; ++w) {
+    for (int w = w0; sums != 0 && w < w1; ++w) {
       uint32_t b[3];
       split(w, &b[0], &b[1], &b[2]);
       const int base = lo + 32 * w;
@@ -543,9 +568,9 @@ struct EvictPlan {
   int64_t list, chunk;     // entries of a list in the workspace (0: never needed) and of all a CTA has there
   size_t bytes;
 };
-constexpr int kMaxFit = 16384;
-constexpr int evict_smem(int fit) { return 12 * fit + 2 * ((fit + 31) / 32) * 4; }
-static_assert(evict_smem(kMaxFit) + kPasses * kBins * 4 + 1024 <= 227 * 1024, "shared memory");
+constexpr int kMaxFit = 20480;
+constexpr int evict_smem(int fit) { return 8 * fit + 2 * ((fit + 31) / 32) * 4; }
+static_assert(evict_smem(kMaxFit) + kHistWords * 4 + 1024 <= 227 * 1024, "shared memory");
 
 // (the counts are on the device: a session that holds more than its budget says, once, is found there)
 static EvictPlan evict_plan(const we_b200_paged_geom& g, int32_t T, int32_t keep) {
