@@ -14,7 +14,7 @@
 // softmax statistics.  A unit that lies in one run is finished there; of one that lies in several each leaves
 // (m, l, O) in the workspace and paged_join_kernel puts them together, in the order of the tokens.
 //
-// One CTA per SM, 384 threads:
+// One CTA per SM, 416 threads:
 //   warps 0-7  softmax, two groups of 128 threads that take tiles in turn, each with statistics and an accumulator of
 //              its own (put together at the end of a segment).  Thread t of a group owns token t of a tile (TMEM
 //              lane t): its logits of the G heads are G columns.  The reference m_g is raised only when a logit
@@ -25,7 +25,8 @@
 //              16-byte stores per token.
 //   warp 8     walks the run and publishes the segments, one ahead of the one being loaded: what to read, its first
 //              pages, its Q rows; takes further runs
-//   warp 11    loads the K and V tiles (a ring each)
+//   warp 11    loads the K tiles, warp 12 the V tiles (a ring each; issuing a copy takes a warp about 0.1 us, and a tile
+//              is four to eight: one warp for both held up the tiles of head dim 64)
 //   warp 9     issues S^T, warp 10 issues O^T (one thread each)
 // Tensor memory (128 columns): four S buffers of 16, O of either group (high and low parts of up to 16 heads: 32).
 #include <cuda_bf16.h>
@@ -37,7 +38,7 @@
 
 namespace we {
 
-constexpr int kPagedThreads = 384;
+constexpr int kPagedThreads = 416;
 constexpr int kPagedWarps = kPagedThreads / 32;
 constexpr int kTile = 128;                 // tokens per tile
 constexpr int kSegs = 3;                   // segments in flight
@@ -149,10 +150,12 @@ struct PagedCfg {
 struct UnitHeads {
   int s, h, hq0, n;          // session, kv head, first query head, query heads
 };
+// (integer divisions cost some fifty cycles each: one unit per kv head is the rule)
+__device__ __forceinline__ int kv_head_of(const PagedAttnParams& p, int u) { return p.chunks == 1 ? u : u / p.chunks; }
 __device__ __forceinline__ UnitHeads unit_heads(const PagedAttnParams& p, int u) {
   UnitHeads r;
-  const int sh = u / p.chunks, c = u - sh * p.chunks;
-  r.s = sh / p.v.Hkv;
+  const int sh = kv_head_of(p, u), c = u - sh * p.chunks;
+  r.s = static_cast<int>(static_cast<uint32_t>(sh) / static_cast<uint32_t>(p.v.Hkv));
   r.h = sh - r.s * p.v.Hkv;
   r.hq0 = r.h * p.group + c * kMaxGroup;
   r.n = min(p.group - c * kMaxGroup, kMaxGroup);
@@ -175,19 +178,22 @@ __device__ void write_empty(const PagedAttnParams& p, int u, int dh) {
 struct Cut {
   int first, later, border, runs;
   __device__ __forceinline__ Cut(const PagedAttnParams& p, int total) {
-    const int share = max((total + p.grid - 1) / p.grid, p.min_share);
+    const int share = max(static_cast<int>(static_cast<uint32_t>(total + p.grid - 1) / static_cast<uint32_t>(p.grid)), p.min_share);
     first = share;
     later = 1;
+    border = total;
+    runs = p.grid;
     // (a run of fewer than 32 tiles ends too soon for the difference to be worth the joins of small ones)
     if (p.dynamic && share >= 32 * p.min_share) {
       first = share - 3 * (share >> 4);
       later = max(share >> 5, 6 * p.min_share);
+      border = static_cast<int>(min(static_cast<int64_t>(first) * p.grid, static_cast<int64_t>(total)));
+      runs += (total - border + later - 1) / later;
     }
-    border = static_cast<int>(min(static_cast<int64_t>(first) * p.grid, static_cast<int64_t>(total)));
-    runs = p.grid + (total - border + later - 1) / later;
   }
   __device__ __forceinline__ int run_of(int granule, int grid) const {
-    return granule < border ? granule / first : grid + (granule - border) / later;
+    return granule < border ? static_cast<int>(static_cast<uint32_t>(granule) / static_cast<uint32_t>(first))
+                            : grid + (granule - border) / later;
   }
   __device__ __forceinline__ int64_t begin(int run, int grid) const {
     return run < grid ? static_cast<int64_t>(run) * first : border + static_cast<int64_t>(run - grid) * later;
@@ -280,7 +286,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     }
     for (int i = 0; i < kSegs; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 11);        // eight softmax warps, both issuers, the loader
+      mbar_init(&q_empty[i], 12);        // eight softmax warps, both issuers, both loaders
     }
     for (int i = 0; i < kBufs; ++i) {
       mbar_init(&s_full[i], 1);
@@ -296,7 +302,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ------------------------------------------------------------------ this CTA's run of granules
-  auto held = [&](int u) { return paged_count(p.v, p.lens[u / p.chunks]); };
+  auto held = [&](int u) { return paged_count(p.v, p.lens[kv_head_of(p, u)]); };
   const int gs = p.gran_shift;
   auto granules = [&](int n) { return (n + (1 << gs) - 1) >> gs; };
   auto cost = [&](int n) { return n > 0 ? granules(n) + p.min_share : 0; };
@@ -329,11 +335,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     }
     if (lane == 31) s_plan[4 + warp] = pre;
     __syncthreads();
-    for (int w = 0; w < kPagedWarps; ++w) {
-      const int y = s_plan[4 + w];
-      if (w < warp) pre += y;
-      total += y;
-    }
+    const int y = lane < kPagedWarps ? s_plan[4 + lane] : 0;
+    total = __reduce_add_sync(0xffffffffu, y);
+    pre += __reduce_add_sync(0xffffffffu, lane < warp ? y : 0);
     pre -= sum;
     if (lane == 0) s_pre[warp] = pre;
     const Cut cut(p, total);
@@ -407,7 +411,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
       while (true) {
         if (left <= 0 && cut.runs > p.grid && run < cut.runs) take_run();
         if (left <= 0 || u >= end_unit) break;
-        n_next = u + 1 < end_unit ? p.lens[(u + 1) / p.chunks] : 0;        // (clamped when its turn comes)
+        n_next = u + 1 < end_unit ? p.lens[kv_head_of(p, u + 1)] : 0;        // (clamped when its turn comes)
         const int head = n > 0 ? max(p.min_share - at, 0) : 0;             // of the unit's head, in this run
         tok0 = max(at - p.min_share, 0) << gs;
         ntok = n - tok0;
@@ -468,8 +472,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
       at = 0;
       n = paged_count(p.v, n_next);
     }
-  } else if (warp == 11) {
-    // ---------------------------------------------------------------- K and V tiles
+  } else if (warp >= 11) {
+    // ---------------------------------------------------------------- K tiles (warp 11) and V tiles (warp 12)
+    const bool is_k = warp == 11;
+    uint64_t* full = is_k ? k_full : v_full;
+    uint64_t* empty = is_k ? k_empty : v_empty;
+    const uint32_t ring = smem_u32(is_k ? sK : sV);
+    const int x_plane = is_k ? 0 : static_cast<int>(p.unit_plane);
     const uint64_t policy = p.chunks == 1 ? l2_evict_first() : l2_evict_normal();
     int it = 0;
     // The first segment is plain from the set-up: its first tiles are asked for while warp 8 still gathers its queries.
@@ -493,7 +502,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&q_empty[qslot]);
-          mbar_arrive(taken);
+          if (is_k) mbar_arrive(taken);
         }
       };
       if (!early) {
@@ -504,25 +513,19 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
         first_pages = PageWalk::fetch(p, row, d.tok0, d.tok0 + d.ntok, lane);
       }
       const UnitHeads w = unit_heads(p, d.unit);
-      const int end = d.tok0 + d.ntok, x_head = w.h * static_cast<int>(p.unit_head);
+      const int end = d.tok0 + d.ntok, x_head = w.h * static_cast<int>(p.unit_head) + x_plane;
       PageWalk walk;
       walk.begin(p, w.s, d.tok0, end, first_pages, lane);
       for (int t0 = d.tok0; t0 < end; t0 += kTile, ++it) {
         const int st = it % C::kStages, ng = (min(kTile, end - t0) + (1 << gs) - 1) >> gs;
         const int pg = walk.page(p, (t0 - d.tok0) / kTile, lane);
-        const int row = ((t0 + (lane << gs)) & (p.v.page - 1)) >> 3, x = pg * static_cast<int>(p.unit_page) + x_head;
-        const uint32_t at = st * C::kTileBytes + lane * ((DH * 2) << gs), parity = ((it / C::kStages) & 1) ^ 1;
-        ok = mbar_wait(&k_empty[st], parity, s_abort);
+        ok = mbar_wait(&empty[st], ((it / C::kStages) & 1) ^ 1, s_abort);
         if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) mbar_arrive_expect_tx(&k_full[st], (ng << gs) * DH * 2);
-        __syncwarp();
-        if (lane < ng) tma_load_5d(smem_u32(sK) + at, &tm, &k_full[st], 0, 0, 0, row, x, policy);
-        ok = mbar_wait(&v_empty[st], parity, s_abort);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        if (lane == 0) mbar_arrive_expect_tx(&v_full[st], (ng << gs) * DH * 2);
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], (ng << gs) * DH * 2);
         __syncwarp();
         if (lane < ng)
-          tma_load_5d(smem_u32(sV) + at, &tm, &v_full[st], 0, 0, 0, row, x + static_cast<int>(p.unit_plane), policy);
+          tma_load_5d(ring + st * C::kTileBytes + lane * ((DH * 2) << gs), &tm, &full[st], 0, 0, 0,
+                      ((t0 + (lane << gs)) & (p.v.page - 1)) >> 3, pg * static_cast<int>(p.unit_page) + x_head, policy);
         if (early) {
           early = false;
           receive();
@@ -770,8 +773,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
           const float m1 = s_join[g], top = fmaxf(m[g], m1);
           const float f0 = exp2_fast(m[g] - top), f1 = exp2_fast(m1 - top);
           m[g] = top;
-          l[g] = l[g] * f0 + s_join[16 + g] * f1;
-          o[g] = o[g] * f0 + other_o[g * 128 + row] * f1;
+          // (which group had the first tile depends on what the CTA did before: the sum must not, so no fused multiply-add)
+          l[g] = __fadd_rn(__fmul_rn(l[g], f0), __fmul_rn(s_join[16 + g], f1));
+          o[g] = __fadd_rn(__fmul_rn(o[g], f0), __fmul_rn(other_o[g * 128 + row], f1));
           lse[g] = m[g] + log2f(l[g]);
         }
       }
