@@ -79,6 +79,46 @@ def test_attention_where_runs_are_handed_out(S, H, G, page, lens):
         assert torch.equal(c.weights.nan_to_num(), first.nan_to_num())
 
 
+@pytest.mark.parametrize("G", [1, 3, 16, 20])
+@pytest.mark.parametrize("page", [16, 64, 128])
+def test_attention_of_sessions_that_are_never_split(G, page):
+    lens = [[(s * 31 + h * 47) % 129 for h in range(3)] for s in range(70)]      # more heads than SMs, some hold nothing
+    c = Cache(70, 3, 128, page, 128 // page, F16, seed=G, lens=lens)
+    q = queries(c, G)
+    lse = torch.empty(70, 3 * G, device="cuda")
+    check_attention(c, q, ops.paged_attn(q, c.kv, c.table, c.lens, lse=lse), lse)
+
+
+def test_pages_beyond_32_bits_of_elements():
+    # offsets of more than 2^31 elements within a plane of the pool, and K and V planes as far apart
+    H, page, Dh = 2, 256, 128
+    P = (1 << 31) // (H * page * Dh) + 40
+    kv = torch.empty(2, P, H, page, Dh, dtype=BF16, device="cuda")
+    weights, positions = torch.zeros(P, H, page, device="cuda"), torch.zeros(P, H, page, dtype=torch.int32, device="cuda")
+    table = torch.tensor([[P - 1, 3, P - 20, P - 7]], dtype=torch.int32, device="cuda")
+    small = Cache(1, H, Dh, page, 4, BF16, seed=2, lens=[0])
+    for far, near in ((kv, small.kv), (weights, small.weights), (positions, small.positions)):
+        if far is kv:
+            far[:, table[0].long()] = near[:, small.table[0].long()]
+        else:
+            far[table[0].long()] = near[small.table[0].long()]
+    lens, next_pos = small.lens.clone(), small.next_pos.clone()
+    for T, keep in ((700, 1000), (600, 1000)):
+        (k, v, w), _ = small.new(T, seed=T, with_weights=True)
+        ops.paged_append_evict_(kv, table, lens, next_pos, k, v, weights, positions, keep, 4, 100, w_new=w)
+        ops.paged_append_evict_(small.kv, small.table, small.lens, small.next_pos, k, v, small.weights, small.positions, keep,
+                                4, 100, w_new=w)
+    q = queries(small, 2)
+    out = ops.paged_attn(q, kv, table, lens, weights=weights)
+    assert torch.equal(out, ops.paged_attn(q, small.kv, small.table, small.lens, weights=small.weights))
+    t, u = table[0].long(), small.table[0].long()
+    assert torch.equal(kv[:, t].view(torch.int16), small.kv[:, u].view(torch.int16))
+    assert torch.equal(weights[t].nan_to_num(), small.weights[u].nan_to_num()) and torch.equal(positions[t], small.positions[u])
+    (k, v, _), _ = small.new(3, seed=9)
+    ops.paged_append_(kv, table, lens, next_pos, k, v)
+    assert torch.equal(kv[0, P - 7, :, 1000 - 768:1003 - 768], k[0].contiguous())
+
+
 @pytest.mark.parametrize("gain", [0.0, 8.0, 40.0])
 def test_attention_with_flat_and_peaked_softmax(gain):
     # gain 40: logits of some hundreds, the running maximum rises many times; 0: all weights equal
@@ -354,6 +394,37 @@ def test_a_captured_step_replays_across_the_budget():
         assert torch.equal(y, want), i
     for name in ("kv", "weights", "positions", "lens", "next_pos"):
         assert torch.equal(getattr(eager, name), getattr(graphed, name)), name
+
+
+def test_a_step_of_everything_on_two_streams():
+    """Two slabs of their own, a step of each on a stream of its own, over and over: as one after the other."""
+    def slab():
+        x = PagedSlab(6, 4, 128, BF16, 32, 6 * 20, 640, keep=600, sink=4, recent=50)
+        for s in range(6):
+            x.reserve(s, 600)
+        return x
+    g = torch.Generator().manual_seed(3)
+    prompt = torch.randn(2, 6, 4, 590, 128, generator=g).to(BF16).cuda()
+    steps = [[torch.randn(6, n, 1, 128, generator=g).to(BF16).cuda() for n in (8, 4, 4)] for _ in range(25)]
+    alone = slab()
+    alone.append(prompt[0], prompt[1])
+    want = [alone.append_and_attend(*x) for x in steps]
+    torch.cuda.synchronize()
+    pair, got = [slab(), slab()], [[], []]
+    streams = [torch.cuda.Stream() for _ in pair]
+    torch.cuda.synchronize()
+    for i, st in enumerate(streams):
+        with torch.cuda.stream(st):
+            pair[i].append(prompt[0], prompt[1])
+    for x in steps:
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(pair[i].append_and_attend(*x))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want))
+        for name in ("kv", "weights", "positions", "lens", "next_pos"):
+            assert torch.equal(getattr(pair[i], name), getattr(alone, name)), name
 
 
 def test_calls_on_two_streams_do_not_disturb_each_other():

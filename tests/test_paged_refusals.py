@@ -118,6 +118,78 @@ def test_ops_refuse_cpu_tensors():
         slab.attend(x)
 
 
+def test_ops_refuse_what_has_a_gradient():
+    slab = PagedSlab(2, 2, 64, torch.bfloat16, 16, 4, 32, device="cpu")
+    x = torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16, requires_grad=True)
+    for call in (lambda: slab.append(x, x), lambda: slab.attend(x)):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+def meta(shape, dtype=torch.bfloat16, stride=None, device=0):
+    t = torch.empty(shape, dtype=dtype, device="meta")
+    return t.shape, t.stride() if stride is None else stride, dtype, device
+
+
+def attn_metas(**kw):
+    m = dict(q=meta((3, 8, 1, 128)), kv=meta((2, 50, 4, 32, 128)), table=meta((3, 10), torch.int32),
+             lens=meta((3, 4), torch.int32), weights=meta((50, 4, 32), torch.float32), out=ops._NONE, lse=ops._NONE)
+    m.update(kw)
+    return m
+
+
+def test_shapes_types_and_devices_of_attention(lib):
+    geom, shape, need = ops._attn_plan(**attn_metas())
+    assert shape == (3, 8, 1, 128) and need > 0 and geom[:6] == (3, 4, 128, 32, 50, 10)
+    for change in (dict(q=meta((3, 8, 2, 128))), dict(q=meta((2, 8, 1, 128))), dict(q=meta((3, 8, 1, 128), torch.float16)),
+                   dict(q=meta((3, 8, 1, 128), stride=(1, 3, 1, 24))), dict(q=meta((3, 8, 128))),
+                   dict(kv=meta((2, 50, 4, 32, 128), stride=(1, 2, 3, 4, 5))), dict(kv=meta((1, 50, 4, 32, 128))),
+                   dict(kv=meta((50, 4, 32, 128))), dict(table=meta((3, 10), torch.int64)), dict(table=meta((10,), torch.int32)),
+                   dict(lens=meta((3,), torch.int32)), dict(lens=meta((3, 4), torch.int64)),
+                   dict(lens=meta((3, 4), torch.int32, stride=(1, 3))), dict(weights=meta((50, 4, 32), torch.float16)),
+                   dict(weights=meta((50, 4, 16), torch.float32)), dict(out=meta((3, 8, 128))),
+                   dict(out=meta((3, 8, 1, 128), torch.float32)), dict(lse=meta((3, 4), torch.float32)),
+                   dict(lens=meta((3, 4), torch.int32, device=1)), dict(q=meta((3, 8, 1, 128), device=1))):
+        with pytest.raises(ValueError):
+            ops._attn_plan(**attn_metas(**change))
+    with pytest.raises(TypeError):
+        ops._attn_plan(**attn_metas(kv=meta((2, 50, 4, 32, 128), torch.float64)))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops._attn_plan(**attn_metas(lens=meta((3, 4), torch.int32, device=-1)))
+
+
+def append_metas(**kw):
+    counts = meta((3, 4), torch.int32)
+    m = dict(kv=meta((2, 50, 4, 32, 128)), table=meta((3, 10), torch.int32), lens=counts, next_pos=counts, lens_out=counts,
+             next_pos_out=counts, k_new=meta((3, 4, 7, 128)), v_new=meta((3, 4, 7, 128)), n_new=meta((3,), torch.int32),
+             weights=meta((50, 4, 32), torch.float32), positions=meta((50, 4, 32), torch.int32),
+             w_new=meta((3, 4, 7), torch.float32))
+    m.update(kw)
+    return m
+
+
+def test_shapes_and_types_of_appends(lib):
+    geom, strides, w_strides, T, need = ops._append_plan(**append_metas())
+    assert T == 7 and need == 0 and strides == (4 * 7 * 128, 7 * 128, 128) * 2 and w_strides == (28, 7, 1)
+    for change in (dict(k_new=meta((3, 4, 6, 128))), dict(v_new=meta((3, 4, 7, 64))), dict(k_new=meta((3, 7, 4, 128))),
+                   dict(v_new=meta((3, 4, 7, 128), torch.float16)), dict(k_new=meta((3, 4, 7, 128), stride=(1, 1, 1, 2))),
+                   dict(n_new=meta((3,), torch.int64)), dict(n_new=meta((4,), torch.int32)), dict(w_new=meta((3, 4, 6), torch.float32)),
+                   dict(w_new=meta((3, 4, 7), torch.bfloat16)), dict(positions=meta((50, 4, 32), torch.int64)),
+                   dict(next_pos=meta((4, 3), torch.int32)), dict(lens_out=meta((3, 4), torch.float32))):
+        with pytest.raises(ValueError):
+            ops._append_plan(**append_metas(**change))
+
+
+@pytest.mark.parametrize("budget", [(0, 0, 0), (-5, 0, 0), (2 ** 31, 0, 0), (10, -1, 0), (10, 0, -1), (10, 6, 5)])
+def test_budgets_that_make_no_sense(budget):
+    slab = PagedSlab(2, 2, 64, torch.bfloat16, 16, 4, 32, device="cpu")
+    x = torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        ops.paged_append_evict_(slab.kv, slab.table, slab.lens, slab.next_pos, x, x, slab.weights, slab.positions, *budget)
+
+
 def test_pages_are_handed_out_once_and_come_back():
     slab = PagedSlab(3, 2, 64, torch.bfloat16, 16, 6, 64, device="cpu")
     slab.reserve(0, 17)
