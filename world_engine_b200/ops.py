@@ -377,7 +377,7 @@ def _append(fn, where, kv, table, lens, next_pos, k_new, v_new, n_new, weights, 
              (positions.shape, positions.stride(), positions.dtype, positions.get_device())),
            *(_NONE if w_new is None else (w_new.shape, w_new.stride(), w_new.dtype, w_new.get_device())), keep)
     geom, strides, w_strides, T, need = _append_plans.get(key) or _plan(_append_plans, _append_plan, key)
-    ws = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
+    ws = kv.new_empty((need + 1) // 2) if need else None          # (in 16-bit values: cheaper to ask for than bytes)
     _call_paged(fn, _lib.PAGED_APPEND_PACK.pack(
         *geom, k_new.data_ptr(), v_new.data_ptr(), *strides, kv.data_ptr(),
         0 if weights is None else weights.data_ptr(), 0 if positions is None else positions.data_ptr(),
@@ -452,7 +452,7 @@ def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: tor
     geom, shape, need = _attn_plans.get(key) or _plan(_attn_plans, _attn_plan, key)
     if out is None:
         out = q.new_empty(shape)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ws = q.new_empty((need + 1) // 2) if need else None            # (in 16-bit values: cheaper to ask for than bytes)
     os_ = out.stride()
     _call_paged(_lib.load().we_b200_paged_attn, _lib.PAGED_ATTN_PACK.pack(
         *geom, q.data_ptr(), out.data_ptr(), qs[0], qs[1], os_[0], os_[1], kv.data_ptr(), table.data_ptr(),
