@@ -365,7 +365,7 @@ typedef struct we_b200_paged_attn_args {
  * token j of kv head h has sum_g p_gj added to its weight; with `lse`, the
  * logarithm of the softmax sum (natural units) is stored.  A head that holds
  * nothing gives 0 and -inf.  Workspace: we_b200_paged_attn_workspace_bytes,
- * contents irrelevant before and after.
+ * contents irrelevant before and after.  out must not overlap q.
  */
 WE_B200_API int we_b200_paged_attn(const we_b200_paged_attn_args* args_host, int32_t* status, void* stream);
 WE_B200_API size_t we_b200_paged_attn_workspace_bytes(const we_b200_paged_geom* geom_host, int32_t Hq,

@@ -160,6 +160,28 @@ def test_attention_takes_strided_tensors_and_a_scale():
     assert torch.equal(ops.paged_attn(q, c.kv, table, c.lens, scale=0.25), out)
 
 
+def test_attention_over_other_orders_of_the_pool():
+    # K and V of a page next to each other, pages last, heads first: any strides will do
+    c = Cache(3, 2, 64, 16, 30, F16, seed=17, lens=[450, 31, 480])
+    q = queries(c, 4)
+    want = ops.paged_attn(q, c.kv, c.table, c.lens)
+    for order in ((1, 0, 2, 3, 4), (2, 1, 0, 3, 4), (3, 1, 2, 0, 4), (2, 3, 0, 1, 4)):
+        back = [order.index(i) for i in range(5)]
+        kv = c.kv.permute(order).contiguous().permute(back)
+        assert kv.shape == c.kv.shape and torch.equal(ops.paged_attn(q, kv, c.table, c.lens), want)
+    with pytest.raises(ValueError, match="out must not"):
+        ops.paged_attn(q, c.kv, c.table, c.lens, out=q)
+
+
+@pytest.mark.parametrize("page,M", [(16, 8), (16, 40)])
+def test_attention_when_nobody_holds_anything(page, M):
+    c = Cache(3, 2, 128, page, M, BF16, seed=18, lens=[0, 0, 0])
+    lse, before = torch.zeros(3, 4, device="cuda"), c.weights.clone()
+    out = ops.paged_attn(queries(c, 2), c.kv, c.table, c.lens, weights=c.weights, lse=lse)
+    assert torch.all(out == 0) and torch.all(torch.isneginf(lse))
+    assert torch.equal(c.weights.nan_to_num(), before.nan_to_num())
+
+
 def test_attention_follows_the_formula_for_infinities_and_nan():
     c = Cache(4, 1, 64, 16, 20, BF16, seed=8, lens=[300, 300, 300, 300])
     q = torch.ones(4, 1, 1, 64, dtype=BF16, device="cuda")

@@ -1,16 +1,16 @@
 // Append to the paged KV cache, without and with a budget (sm_100a).
 //
 // Both give every (session, kv head) to a thread-block cluster of 1 to 8 CTAs, which alone reads and writes its counts,
-// so they can be updated in place.  The append is a copy of rows: 16 bytes per thread and plane, all loads of a thread
-// under way before the first store.
+// so they can be updated in place.  The append is a copy of rows: 16 bytes per thread and plane.
 //
 // Under a budget the cluster first finds the key of the last token to keep: weights are mapped to unsigned numbers of
-// the same order (shielded tokens above all) and the keep-th largest is found digit by digit, each CTA counting
-// the digits of its slice of the candidates and adding up the other CTAs' counts through cluster shared memory.  One
-// pass over weights and positions in global memory: the keys stay in registers (those of longer slices are read again
-// for every digit).  Then each CTA lists, in the order of the indexes, the holes of its slice
-// (indexes below the budget that are given up) and the movers (kept ones behind it), and the j-th mover goes to the
-// j-th hole: as many rows are copied as tokens leave, not as many as stay.
+// the same order (shielded tokens above all) and the keep-th largest is found digit by digit, each CTA counting the
+// digits of its slice of the candidates and adding up the other CTAs' counts through cluster shared memory.  Weights and
+// positions are read once: the keys stay in registers (those of longer slices are read again for every digit).  Then
+// each CTA lists, in the order of the indexes, the holes of its slice (indexes below the budget that are given up) and
+// the movers (kept ones behind it), and the j-th mover goes to the j-th hole: as many rows are copied as tokens leave,
+// not as many as stay.  Reading is a matter of 1 to 3 us; what bounds the kernel is the chain of its phases (11 to
+// 20 us): counts -> table -> keys -> two or three digits -> lists -> table -> rows, with a barrier or two in each.
 #include "paged.cuh"
 
 namespace we {
@@ -18,8 +18,8 @@ namespace we {
 constexpr int kAppendThreads = 256;
 constexpr int kMaxCluster = 8;
 // Candidates a CTA deals with before its (session, head) gets a cluster: a barrier of the cluster and the counts read
-// through it cost about 2 us a digit, 4096 more candidates in one CTA less (16 heads of 4097: 12.9 us in one CTA,
-// 14.3 in two; 16 heads of 17001: 20.9 us in four CTAs, 28 in eight, which do not all find room at once).
+// through it cost 1 to 2 us a digit, 4096 more candidates in one CTA less (16 heads of 4097: 11.2 us in one CTA, 14.6
+// in two; 16 heads of 17001: 18.3 us in four CTAs, 31.9 in eight, which do not all find room at once).
 constexpr int kEvictPerCta = 8192;
 
 struct PagedAppendParams {
@@ -42,7 +42,7 @@ struct PagedAppendParams {
   int32_t T, keep, sink, recent;
   int32_t vec_shift;     // log2 of 16-byte vectors per row
   int32_t cluster;       // CTAs per (session, head)
-  int32_t fit;           // keys of a slice that fit in shared memory
+  int32_t fit;           // entries of a list that fit in shared memory
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -137,9 +137,12 @@ __device__ __forceinline__ void move_tokens(const PagedAppendParams& p, int s, i
   }
 }
 
-// (five CTAs on an SM with two rows under way per thread: 29.8 us for prompts of 142000 rows; three with four: 32.3,
-// eight with one: 34.1)
-__global__ void __launch_bounds__(kAppendThreads, 5) paged_append_kernel(const PagedAppendParams p) {
+// 16-byte vectors of K and of V that a thread has under way (and the pages of its next ones).  Prompts of 142000 tokens
+// (146 MB read and written): 28.1 us with two and six CTAs on an SM, 5.2 TB/s or 0.79 of the measured copy; 30.3 with
+// five, 34.8 with one vector and eight CTAs, 30.9 with four and four.  Bound by the latency of the rows' loads.
+constexpr int kRows = 2;
+
+__global__ void __launch_bounds__(kAppendThreads, 6) paged_append_kernel(const PagedAppendParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int unit = blockIdx.x / p.cluster, rank = blockIdx.x - unit * p.cluster;
@@ -150,8 +153,49 @@ __global__ void __launch_bounds__(kAppendThreads, 5) paged_append_kernel(const P
   const int room = (p.v.max_pages << p.v.page_shift) - len;
   const int take = n < room ? n : room;
   if (take < n && threadIdx.x == 0) paged_report(p.v);
-  move_tokens<2>(p, s, h, len, pos0, take, rank * blockDim.x + threadIdx.x, p.cluster * blockDim.x,
-                 [&](int e, int* src, int* dst) { *src = *dst = len + e; });
+  const int32_t* table = p.v.table + s * p.v.table_stride;
+  const int c = threadIdx.x & ((1 << p.vec_shift) - 1);
+  const uint16_t* k_new = p.k_new + s * p.ks[0] + h * p.ks[1] + 8 * c;
+  const uint16_t* v_new = p.v_new + s * p.vs[0] + h * p.vs[1] + 8 * c;
+  uint16_t* kv = p.kv + h * p.v.head_s + 8 * c;
+  const int step = (p.cluster * static_cast<int>(blockDim.x)) >> p.vec_shift;            // tokens
+  int t0 = (rank * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) >> p.vec_shift;
+  auto page_of = [&](int t) { return t < take ? table[(len + t) >> p.v.page_shift] : -1; };
+  int pg[kRows];
+#pragma unroll
+  for (int d = 0; d < kRows; ++d) pg[d] = page_of(t0 + step * d);
+  for (; t0 < take; t0 += step * kRows) {
+    uint4 k[kRows], v[kRows];
+    int next[kRows];
+#pragma unroll
+    for (int d = 0; d < kRows; ++d) {
+      const int t = t0 + step * d;
+      if (t >= take) continue;
+      k[d] = *reinterpret_cast<const uint4*>(k_new + t * p.ks[2]);
+      v[d] = *reinterpret_cast<const uint4*>(v_new + t * p.vs[2]);
+    }
+#pragma unroll
+    for (int d = 0; d < kRows; ++d) next[d] = page_of(t0 + step * (kRows + d));
+#pragma unroll
+    for (int d = 0; d < kRows; ++d) {
+      const int t = t0 + step * d, row = (len + t) & (p.v.page - 1);
+      if (t >= take) continue;
+      if (pg[d] < 0 || pg[d] >= p.v.n_pages) {
+        paged_report(p.v);
+        continue;
+      }
+      uint16_t* dst = kv + pg[d] * p.v.page_s + row * p.v.token_s;
+      *reinterpret_cast<uint4*>(dst) = k[d];
+      *reinterpret_cast<uint4*>(dst + p.v.plane_s) = v[d];
+      if (c == 0) {
+        const int64_t m = meta_index(p, pg[d], h, row);
+        if (p.weights != nullptr) p.weights[m] = new_weight(p, s, h, t);
+        if (p.positions != nullptr) p.positions[m] = pos0 + t;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < kRows; ++d) pg[d] = next[d];
+  }
   unit_sync(p);                          // every thread has read the counts before they are replaced
   if (threadIdx.x == 0 && rank == 0) {
     p.lens_out[unit] = len + take;
@@ -576,8 +620,8 @@ static_assert(evict_smem(kMaxFit) + kHistWords * 4 + 1024 <= 227 * 1024, "shared
 static EvictPlan evict_plan(const we_b200_paged_geom& g, int32_t T, int32_t keep) {
   EvictPlan r;
   const int64_t units = static_cast<int64_t>(g.S) * g.Hkv, usual = static_cast<int64_t>(keep) + T;
-  // four CTAs of 256 threads fit on an SM, or one of 512 has it to itself (one head of 4097: 15.5 us with 256 threads,
-  // 12.9 with 512, 13.6 with 1024, whose scans over the block take longer; 512 heads of 2064: 13.5 us, 16.4 with 512)
+  // four CTAs of 256 threads fit on an SM, or one of 512 has it to itself (16 heads of 4097: 15.5 us with 256 threads,
+  // 12.9 with 512, 13.6 with 1024, whose scans over the block take longer; 512 heads of 2064: 13.1 us, 16.4 with 512)
   r.threads = units > 2 * sm_count() ? 256 : 512;
   r.cluster = cluster_for(units, usual, kEvictPerCta, sm_count());
   const int64_t fit = ((usual + r.cluster - 1) / r.cluster + 3) & ~3ll;

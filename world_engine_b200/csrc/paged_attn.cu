@@ -345,7 +345,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     if (tid == 0) s_plan[2] = g0 < cut.border ? static_cast<int>(min(static_cast<int64_t>(cut.first), cut.border - g0)) : 0;
     if (g0 >= pre && g0 < pre + sum) {
       int u = first, at = pre;
-      for (int n = cost(held(u)); at + n <= g0; n = cost(held(++u))) at += n;
+      for (int n = cost(held(u)); at + n <= g0 && u + 1 < last; n = cost(held(++u))) at += n;
       s_plan[0] = u;
       s_plan[1] = static_cast<int>(g0) - at;
       s_plan[3] = held(u);

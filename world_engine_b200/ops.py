@@ -438,7 +438,8 @@ def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: tor
     """Attention of one new token per session over its paged cache (we_b200_paged_attn).  `q` is a
     `[S, Hq, 1, Dh]` view; the output has its shape.  With `weights` the softmax weight every held token is given
     (summed over the query heads of its kv head) is added to it in place; `lse` (float32 `[S, Hq]`, contiguous)
-    receives the logarithm of the softmax sum.  A kv head that holds nothing gives 0 and -inf."""
+    receives the logarithm of the softmax sum.  A kv head that holds nothing gives 0 and -inf.  `out` must not overlap
+    `q`.  Results repeat bit for bit (but for the weights of pages that several sessions share)."""
     if torch.is_grad_enabled():
         _refuse_grad(q, kv, weights, out, lse)
     index, qs = q.get_device(), q.stride()
@@ -451,7 +452,9 @@ def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: tor
            *(_NONE if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.get_device())))
     geom, shape, need = _attn_plans.get(key) or _plan(_attn_plans, _attn_plan, key)
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q)
+    elif out.data_ptr() == q.data_ptr():
+        raise ValueError("out must not be q itself: a head's query is read by several CTAs, not all at the same time")
     ws = q.new_empty((need + 1) // 2) if need else None            # (in 16-bit values: cheaper to ask for than bytes)
     os_ = out.stride()
     _call_paged(_lib.load().we_b200_paged_attn, _lib.PAGED_ATTN_PACK.pack(
