@@ -109,6 +109,28 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Sums of N values over a warp, N shuffles and log2(32 / N) more in place of 5 N: at each step a lane keeps one half of
+// its values and gives the other away.  Lane i ends with the sum number i / (32 / N) in v[0].
+template <int N>
+__device__ __forceinline__ void warp_sums(float (&v)[N], int lane) {
+  int d = 16;
+#pragma unroll
+  for (int n = N / 2; n >= 1; n /= 2, d /= 2) {
+    const bool up = (lane & d) != 0;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+    }
+  }
+#pragma unroll
+  for (int k = 32 / N / 2; k >= 1; k /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], k);
+}
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ bool bar_any(int id, int n, bool x) {
   uint32_t r;
@@ -141,7 +163,7 @@ struct PagedCfg {
   static constexpr int kOffP = kOffQ + kSegs * kQBytes;
   static constexpr int kOffAux = kOffP + 2 * kPBytes;
   static constexpr int kAux = 384 + 2 * 512 + 192 + 128 + kSegs * (16 + 128);
-  static_assert((4 * kStages + 2 * kSegs + 2 * kBufs + 3) * 8 <= 384, "barriers");
+  static_assert((4 * kStages + 2 * kSegs + 2 * kBufs + 5) * 8 <= 384, "barriers");
   static constexpr int kSmem = kOffAux + kAux + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -262,6 +284,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   uint64_t* p_full = s_full + kBufs;
   uint64_t* pv_done = p_full + kBufs;
   uint64_t* taken = pv_done + 2;
+  uint64_t* half_full = taken + 1;       // group 1's part of a segment is in shared memory ...
+  uint64_t* half_read = taken + 2;       // ... and group 0 has it
   float* s_max = reinterpret_cast<float*>(aux + 384);                 // [2 groups][4 warps][16]
   float* s_sum = s_max + 128;                                         // [2 groups][4 warps][16]
   float* s_join = s_sum + 128;                                        // group 1's m and l: [2][16]
@@ -295,6 +319,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     mbar_init(&pv_done[0], 1);
     mbar_init(&pv_done[1], 1);
     mbar_init(taken, 1);
+    mbar_init(half_full, 128);
+    mbar_init(half_read, 128);
     *s_abort = 0;
     fence_mbar_init();
   }
@@ -604,12 +630,15 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
     float* other_o = reinterpret_cast<float*>(sP + C::kPBytes);         // [GP][128], in group 1's P buffer
     uint8_t* p_row = sP + grp * C::kPBytes + row * C::kPRow;
     const uint32_t swz = C::kPRow == 32 ? (row >> 2) & 1 : (row >> 1) & 3;
-    int it = 0;
+    int it = 0, halves = 0;
+    bool given = false;                                    // group 1: its part has not been collected yet
+    // (the groups meet nowhere but in segments of several tiles, through barriers with a limit: short segments go to
+    // either group in turn, two at a time)
     for (int seg = 0;; ++seg) {
       const int qslot = seg % kSegs;
       const bool ok = mbar_wait(&q_full[qslot], (seg / kSegs) & 1, s_abort);
       __syncwarp();
-      if (bar_any(1, 256, !ok)) break;
+      if (bar_any(2 + grp, 128, !ok)) break;
       const Segment d = segs[qslot];
       if (d.ntok == 0) break;
       const UnitHeads w = unit_heads(p, d.unit);
@@ -654,8 +683,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
         if (bar_any(2 + grp, 128, over > kRaise)) {
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
-            float t = x[g];
-            for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+            const float t = warp_max(x[g]);
             if (lane == 0) my_max[(warp & 3) * 16 + g] = t;
           }
           bar_sync(2 + grp, 128);
@@ -703,6 +731,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
           }
         }
         if (it >= 2) mbar_wait(&pv_done[grp], ((it - 2) >> 1) & 1, s_abort);      // the P before was read
+        if (given) {
+          mbar_wait(half_read, (halves - 1) & 1, s_abort);
+          given = false;
+        }
         if constexpr (GP == 1) {
           *reinterpret_cast<uint32_t*>(p_row + (swz << 4)) = words[0];
         } else if constexpr (GP == 2) {
@@ -729,45 +761,45 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
         mbar_arrive(&p_full[it % kBufs]);
         last = it;
       }
+      if (last < 0) {                                      // one tile, and the other group had it
+        if (lane == 0) mbar_arrive(&q_empty[qslot]);
+        continue;
+      }
       // ---- the segment's sums: of either group, then of both
+      warp_sums<GP>(l, lane);
+      if (lane % (32 / GP) == 0) my_sum[(warp & 3) * 16 + lane / (32 / GP)] = l[0];
+      bar_sync(2 + grp, 128);
+#pragma unroll
+      for (int g = 0; g < GP; ++g) l[g] = (my_sum[g] + my_sum[16 + g]) + (my_sum[32 + g] + my_sum[48 + g]);
+      mbar_wait(&pv_done[grp], (last >> 1) & 1, s_abort);
+      __syncwarp();
+      tc_fence_after();
+      uint32_t hi[GP], lo[GP];
+      tmem_ld_n<GP>(o_col, hi);
+      tmem_ld_n<GP>(o_col + GP, lo);
+      tmem_ld_wait();
       float o[GP];
 #pragma unroll
-      for (int g = 0; g < GP; ++g) o[g] = 0.f;
-      if (last >= 0) {                                     // (the same for the whole group)
-#pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          for (int k = 16; k > 0; k >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], k);
-          if (lane == 0) my_sum[(warp & 3) * 16 + g] = l[g];
-        }
-        bar_sync(2 + grp, 128);
-#pragma unroll
-        for (int g = 0; g < GP; ++g) l[g] = (my_sum[g] + my_sum[16 + g]) + (my_sum[32 + g] + my_sum[48 + g]);
-        mbar_wait(&pv_done[grp], (last >> 1) & 1, s_abort);
-        __syncwarp();
-        tc_fence_after();
-        uint32_t hi[GP], lo[GP];
-        tmem_ld_n<GP>(o_col, hi);
-        tmem_ld_n<GP>(o_col + GP, lo);
-        tmem_ld_wait();
-#pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          // (an infinite value times a low part, which may be 0 or negative, is none of the formula's terms)
-          const float y = __uint_as_float(lo[g]);
-          o[g] = __uint_as_float(hi[g]) + (fabsf(y) < INFINITY ? y : 0.f);
-        }
+      for (int g = 0; g < GP; ++g) {
+        // (an infinite value times a low part, which may be 0 or negative, is none of the formula's terms)
+        const float y = __uint_as_float(lo[g]);
+        o[g] = __uint_as_float(hi[g]) + (fabsf(y) < INFINITY ? y : 0.f);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_empty[qslot]);
-      if (grp == 1) {
+      if (d.ntok > kTile) {                                // both groups had tiles: group 0 finishes
+        ++halves;
+        if (grp == 1) {
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          other_o[g * 128 + row] = o[g];
-          if (row == g) s_join[g] = m[g], s_join[16 + g] = l[g];
+          for (int g = 0; g < GP; ++g) {
+            other_o[g * 128 + row] = o[g];
+            if (row == g) s_join[g] = m[g], s_join[16 + g] = l[g];
+          }
+          mbar_arrive(half_full);
+          given = true;                                    // (its P buffer, where O lies, is not written until then)
+          continue;
         }
-      }
-      bar_sync(1, 256);
-      float lse[GP];
-      if (grp == 0) {
+        mbar_wait(half_full, (halves - 1) & 1, s_abort);
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
           const float m1 = s_join[g], top = fmaxf(m[g], m1);
@@ -776,23 +808,21 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
           // (which group had the first tile depends on what the CTA did before: the sum must not, so no fused multiply-add)
           l[g] = __fadd_rn(__fmul_rn(l[g], f0), __fmul_rn(s_join[16 + g], f1));
           o[g] = __fadd_rn(__fmul_rn(o[g], f0), __fmul_rn(other_o[g * 128 + row], f1));
-          lse[g] = m[g] + log2f(l[g]);
         }
+        mbar_arrive(half_read);
       }
-      bar_sync(1, 256);                                    // group 1's buffer may be written again
-      if (grp == 0) {
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          if (g >= w.n) continue;
-          if (d.slot >= 0) {
-            if (row < DH) p.ws_o[(static_cast<int64_t>(d.slot) * GP + g) * DH + row] = o[g];
-            if (row == g) p.ws_ml[d.slot * GP + g] = make_float2(m[g], l[g]);
-          } else {
-            if (row < DH) p.out[w.s * p.os[0] + (w.hq0 + g) * p.os[1] + row] = narrow<BF16>(o[g] / l[g]);
-            if (row == g) {
-              if (p.lse != nullptr) p.lse[static_cast<int64_t>(w.s) * p.Hq + w.hq0 + g] = lse[g] * 0.6931471805599453f;
-              if (xs != nullptr) p.ws_lse[static_cast<int64_t>(d.unit) * GP + g] = lse[g];
-            }
+      for (int g = 0; g < GP; ++g) {
+        if (g >= w.n) continue;
+        if (d.slot >= 0) {
+          if (row < DH) p.ws_o[(static_cast<int64_t>(d.slot) * GP + g) * DH + row] = o[g];
+          if (row == g) p.ws_ml[d.slot * GP + g] = make_float2(m[g], l[g]);
+        } else {
+          if (row < DH) p.out[w.s * p.os[0] + (w.hq0 + g) * p.os[1] + row] = narrow<BF16>(o[g] / l[g]);
+          if (row == g && (p.lse != nullptr || xs != nullptr)) {
+            const float lse = m[g] + log2f(l[g]);
+            if (p.lse != nullptr) p.lse[static_cast<int64_t>(w.s) * p.Hq + w.hq0 + g] = lse * 0.6931471805599453f;
+            if (xs != nullptr) p.ws_lse[static_cast<int64_t>(d.unit) * GP + g] = lse;
           }
         }
       }
