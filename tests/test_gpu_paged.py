@@ -119,6 +119,17 @@ def test_pages_beyond_32_bits_of_elements():
     assert torch.equal(kv[0, P - 7, :, 1000 - 768:1003 - 768], k[0].contiguous())
 
 
+@pytest.mark.parametrize("S,H", [(13, 32), (25, 16), (96, 4), (385, 1), (103, 8), (416, 2), (417, 3), (5, 250)])
+def test_attention_at_every_share_of_the_set_up(S, H):
+    # as many heads as the set-up has threads, a few less, more, and multiples of them
+    lens = [[(s * 37 + h * 11) % 150 for h in range(H)] for s in range(S)]
+    c = Cache(S, H, 64, 16, 10, BF16, seed=S, lens=lens)
+    q = queries(c, 1)
+    before = c.w64.copy()
+    lse = torch.empty(S, H, device="cuda")
+    check_attention(c, q, ops.paged_attn(q, c.kv, c.table, c.lens, weights=c.weights, lse=lse), lse, before, c.weights)
+
+
 @pytest.mark.parametrize("gain", [0.0, 8.0, 40.0])
 def test_attention_with_flat_and_peaked_softmax(gain):
     # gain 40: logits of some hundreds, the running maximum rises many times; 0: all weights equal

@@ -221,8 +221,8 @@ struct Cut {
     return run < grid ? static_cast<int64_t>(run) * first : border + static_cast<int64_t>(run - grid) * later;
   }
 };
-// Runs there can be at most, per CTA: its own and 3/16 of a share in pieces of 1/32 of it, rounded down to no less than
-// 32 / 33 of that.
+// Runs there can be at most, per CTA: its own and 3/16 of a share in pieces of 1/32 of it (six of them, rounded down by
+// 1 in 24 at most).
 constexpr int kRunsPerCta = 8;
 
 // The pages of a segment's granules, for the warp that loads tiles: 32 granules (four or eight tiles) per look-up of the
@@ -290,7 +290,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
   float* s_sum = s_max + 128;                                         // [2 groups][4 warps][16]
   float* s_join = s_sum + 128;                                        // group 1's m and l: [2][16]
   int* s_plan = reinterpret_cast<int*>(aux + 1600);                   // 0 unit, 1 granule, 2 run, 3 held, 4.. scan
-  int* s_pre = s_plan + 16;                                           // [warps] granules before the units of a warp
+  int* s_pre = s_plan + 4 + kPagedWarps;                              // [warps] granules before the units of a warp
+  static_assert(4 + 2 * kPagedWarps <= 30, "the set-up's words");
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_plan + 30);
   Segment* segs = reinterpret_cast<Segment*>(aux + 1728);
   int* s_pages = reinterpret_cast<int*>(aux + 1728 + kSegs * 16);     // [segments][32]
