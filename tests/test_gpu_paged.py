@@ -337,6 +337,30 @@ def test_long_budgets(S, H, lens, T, keep, sink, recent):
         c.assert_same_state()
 
 
+@pytest.mark.parametrize("S,H,keep,T", [(100, 3, 5300, 9), (40, 2, 11000, 50), (3, 1, 70001, 3)])
+def test_a_session_does_not_depend_on_its_batch(S, H, keep, T):
+    # many heads: small CTAs that go through their candidates in rounds; one session alone: larger ones, or a cluster
+    page, Dh = 64, 64
+    M = -(-keep // page)
+    g = torch.Generator(device="cuda").manual_seed(S)
+    table = torch.randperm(S * M, generator=g, device="cuda").view(S, M).int()
+    kv = torch.randn(2, S * M, H, page, Dh, generator=g, device="cuda", dtype=BF16)
+    weights = torch.rand(S * M, H, page, generator=g, device="cuda").mul_(64).floor_()           # a few values: many ties
+    positions = torch.randint(0, 2 * keep, (S * M, H, page), generator=g, device="cuda", dtype=torch.int32)
+    lens = torch.full((S, H), keep, dtype=torch.int32, device="cuda")
+    next_pos = torch.full((S, H), 2 * keep, dtype=torch.int32, device="cuda")
+    new = torch.randn(2, S, H, T, Dh, generator=g, device="cuda", dtype=BF16)
+    w_new = torch.rand(S, H, T, generator=g, device="cuda") * 64
+    both = [[x.clone() for x in (kv, lens, next_pos, weights, positions)] for _ in range(2)]
+    a, b = both
+    ops.paged_append_evict_(a[0], table, a[1], a[2], new[0], new[1], a[3], a[4], keep, 5, keep // 50, w_new=w_new)
+    for s in range(S):
+        ops.paged_append_evict_(b[0], table[s:s + 1], b[1][s:s + 1], b[2][s:s + 1], new[0, s:s + 1], new[1, s:s + 1], b[3], b[4],
+                                keep, 5, keep // 50, w_new=w_new[s:s + 1])
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert torch.all(a[1] == keep) and torch.all(a[2] == 2 * keep + T) and not torch.equal(a[4], positions)
+
+
 @pytest.mark.parametrize("padded", [[3, 0, 7], [0, 0, 0], [7, 7, 1]])
 def test_padded_batch_under_a_budget(padded):
     c = Cache(3, 2, 64, 16, 5, BF16, seed=9, lens=[[60, 64], [64, 64], [10, 61]], nhd=True)
@@ -476,12 +500,13 @@ def test_calls_on_two_streams_do_not_disturb_each_other():
         assert all(torch.equal(y, want[i]) for y in got[i])
 
 
-def test_traces_as_one_graph():
-    slab = PagedSlab(2, 2, 64, BF16, 16, 8, 32, keep=20, sink=1, recent=4)
-    ref = PagedSlab(2, 2, 64, BF16, 16, 8, 32, keep=20, sink=1, recent=4)
+@pytest.mark.parametrize("budget", [dict(), dict(keep=20, sink=1, recent=4)])
+def test_traces_as_one_graph(budget):
+    slab = PagedSlab(2, 2, 64, BF16, 16, 8, 32, **budget)
+    ref = PagedSlab(2, 2, 64, BF16, 16, 8, 32, **budget)
     for s in range(2):
-        slab.reserve(s, 20)
-        ref.reserve(s, 20)
+        slab.reserve(s, 30)
+        ref.reserve(s, 30)
     step = torch.compile(lambda q, k, v: slab.append_and_attend(q * 2, k, v) + 1, fullgraph=True, backend="aot_eager")
     g = torch.Generator().manual_seed(6)
     for _ in range(25):

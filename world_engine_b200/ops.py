@@ -332,7 +332,11 @@ def _plan(plans, make, key):
     """The plan of a call nobody made before (a plan depends on nothing but the values in its key)."""
     if len(plans) >= _MAX_PLANS:
         plans.clear()
-    plans[key] = plan = make(*(key[i:i + 4] for i in range(0, len(key) // 4 * 4, 4)), *key[len(key) // 4 * 4:])
+    args = (*(key[i:i + 4] for i in range(0, len(key) // 4 * 4, 4)), *key[len(key) // 4 * 4:])
+    if key[3] < 0:                       # not on a GPU: refused in there
+        return make(*args)
+    with torch.cuda.device(key[3]):      # (a workspace's size depends on the device's SMs)
+        plans[key] = plan = make(*args)
     return plan
 
 
