@@ -297,6 +297,8 @@ def _check_paged(kv, table, counts, per_slot, others) -> Tuple[int, ...]:
         raise ValueError("table must be int32 [S, max_pages] with contiguous rows")
     S, M = table[0]
     for meta in counts:
+        if meta == _NONE:
+            continue
         if meta[2] != torch.int32 or meta[0] != (S, Hkv) or not _dense(meta):
             raise ValueError("token counts and positions must be contiguous int32 [S, Hkv]")
     for meta, want in zip(per_slot, (torch.float32, torch.int32)):
@@ -362,8 +364,6 @@ def _append_plan(kv, table, lens, next_pos, lens_out, next_pos_out, k_new, v_new
 
 def _append(fn, where, kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new, lens_out,
             next_pos_out, keep, sink, recent) -> None:
-    lens_out = lens if lens_out is None else lens_out
-    next_pos_out = next_pos if next_pos_out is None else next_pos_out
     if torch.is_grad_enabled():
         _refuse_grad(kv, k_new, v_new, weights, w_new)
     index = kv.get_device()
@@ -371,8 +371,9 @@ def _append(fn, where, kv, table, lens, next_pos, k_new, v_new, n_new, weights, 
            table.shape, table.stride(), table.dtype, table.get_device(),
            lens.shape, lens.stride(), lens.dtype, lens.get_device(),
            next_pos.shape, next_pos.stride(), next_pos.dtype, next_pos.get_device(),
-           lens_out.shape, lens_out.stride(), lens_out.dtype, lens_out.get_device(),
-           next_pos_out.shape, next_pos_out.stride(), next_pos_out.dtype, next_pos_out.get_device(),
+           *(_NONE if lens_out is None else (lens_out.shape, lens_out.stride(), lens_out.dtype, lens_out.get_device())),
+           *(_NONE if next_pos_out is None else
+             (next_pos_out.shape, next_pos_out.stride(), next_pos_out.dtype, next_pos_out.get_device())),
            k_new.shape, k_new.stride(), k_new.dtype, k_new.get_device(),
            v_new.shape, v_new.stride(), v_new.dtype, v_new.get_device(),
            *(_NONE if n_new is None else (n_new.shape, n_new.stride(), n_new.dtype, n_new.get_device())),
@@ -385,7 +386,8 @@ def _append(fn, where, kv, table, lens, next_pos, k_new, v_new, n_new, weights, 
     _call_paged(fn, _lib.PAGED_APPEND_PACK.pack(
         *geom, k_new.data_ptr(), v_new.data_ptr(), *strides, kv.data_ptr(),
         0 if weights is None else weights.data_ptr(), 0 if positions is None else positions.data_ptr(),
-        table.data_ptr(), lens.data_ptr(), next_pos.data_ptr(), lens_out.data_ptr(), next_pos_out.data_ptr(),
+        table.data_ptr(), lens.data_ptr(), next_pos.data_ptr(), (lens if lens_out is None else lens_out).data_ptr(),
+        (next_pos if next_pos_out is None else next_pos_out).data_ptr(),
         0 if n_new is None else n_new.data_ptr(), 0 if w_new is None else w_new.data_ptr(), *w_strides,
         0 if ws is None else ws.data_ptr(), need, T, keep, sink, recent), index, where)
 
