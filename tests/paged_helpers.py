@@ -99,7 +99,7 @@ def check_attention(c, q, out, lse=None, weights_before=None, weights_after=None
                 vmax[s, h * G:(h + 1) * G] = n * np.abs(c.kv64[1, pg, h, row]).max()
     tol = (u + 2 * dx[..., None] + 2.0 ** -18) * spread + u * np.abs(want)
     if c.dtype == torch.float16:
-        tol = tol + 2.0 ** -25 * vmax[..., None] / np.maximum(1.0, 1.0) + 2.0 ** -25
+        tol = tol + 2.0 ** -25 * vmax[..., None] + 2.0 ** -25
     got = out[:, :, 0].double().cpu().numpy()
     assert np.all(np.isfinite(got))
     worst = np.max(np.abs(got - want) / np.maximum(tol, 1e-300))

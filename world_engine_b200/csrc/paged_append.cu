@@ -273,6 +273,13 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) paged_appen
   const Digits digits(p.cluster);
   const int bins = 1 << digits.bits;
   for (int b = tid; b < digits.passes * bins / 4; b += kThreads) reinterpret_cast<uint4*>(s_hist)[b] = make_uint4(0u, 0u, 0u, 0u);
+  // One CTA starts at the first token whatever the counts are: its pages are looked up while they are on their way.
+  int early[kGroups];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    const int b = (4 * (g * kThreads + tid)) >> p.v.page_shift;
+    early[g] = p.cluster == 1 && b < p.v.max_pages ? p.v.table[s * p.v.table_stride + b] : 0;
+  }
   const int len = paged_count(p.v, p.lens[unit]);
   const int pos0 = p.next_pos[unit];
   const int n = new_count(p, s);
@@ -298,7 +305,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) paged_appen
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         const int i = first_of(round, g);
-        pg[g] = i < hi && i < len ? p.v.table[s * p.v.table_stride + (i >> p.v.page_shift)] : 0;
+        if (p.cluster == 1 && round == 0) pg[g] = early[g];
+        else pg[g] = i < hi && i < len ? p.v.table[s * p.v.table_stride + (i >> p.v.page_shift)] : 0;
       }
 #pragma unroll
       for (int g0 = 0; g0 < kGroups; g0 += kBatch) {
@@ -621,7 +629,7 @@ static EvictPlan evict_plan(const we_b200_paged_geom& g, int32_t T, int32_t keep
   EvictPlan r;
   const int64_t units = static_cast<int64_t>(g.S) * g.Hkv, usual = static_cast<int64_t>(keep) + T;
   // four CTAs of 256 threads fit on an SM, or one of 512 has it to itself (16 heads of 4097: 15.5 us with 256 threads,
-  // 12.9 with 512, 13.6 with 1024, whose scans over the block take longer; 512 heads of 2064: 13.1 us, 16.4 with 512)
+  // 12.9 with 512, 13.6 with 1024, whose scans over the block take longer; 512 heads of 2064: 12.5 us, 16.4 with 512)
   r.threads = units > 2 * sm_count() ? 256 : 512;
   r.cluster = cluster_for(units, usual, kEvictPerCta, sm_count());
   const int64_t fit = ((usual + r.cluster - 1) / r.cluster + 3) & ~3ll;
