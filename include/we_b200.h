@@ -323,7 +323,9 @@ typedef struct we_b200_paged_append_args {
  * Appends n_new[s] tokens to every kv head of session s: token t goes to slot
  * lens[s][h] + t, its weight becomes w_new or 0, its position next_pos[s][h] + t.
  * lens_out / next_pos_out receive the counts after it.  Rows t >= n_new[s] of
- * the new tokens are not read (a padded batch).
+ * the new tokens are not read (a padded batch).  The first token for which the
+ * table names no page (or has no entry left) is dropped with all behind it, and
+ * reported: lens_out counts the tokens before it, next_pos_out all n_new[s].
  */
 WE_B200_API int we_b200_paged_append(const we_b200_paged_append_args* args_host, int32_t* status, void* stream);
 
@@ -336,7 +338,8 @@ WE_B200_API int we_b200_paged_append(const we_b200_paged_append_args* args_host,
  * index.  Kept tokens of an index >= keep move to the indexes < keep that the
  * evicted ones left, both in ascending order; the others stay where they are,
  * so little is moved.  What an evicted slot beyond the budget holds is left as
- * it was.  The workspace (we_b200_paged_evict_workspace_bytes) needs no
+ * it was.  A token whose slot would lie below the budget is dropped where the
+ * table names no page for it, as above.  The workspace (we_b200_paged_evict_workspace_bytes) needs no
  * initialisation.  max_pages * page + T < 2^21.
  */
 WE_B200_API int we_b200_paged_append_evict(const we_b200_paged_append_args* args_host, int32_t* status, void* stream);

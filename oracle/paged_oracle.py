@@ -12,6 +12,19 @@ def slot(table, s, i, page):
     return int(table[s, i // page]), i % page
 
 
+def named(table, s, b, pages):
+    """Whether the table names a page of the pool for block b of session s."""
+    return 0 <= int(table[s, b]) < pages
+
+
+def with_a_page(table, s, first, want, page, pages):
+    """How many of `want` tokens from slot `first` on can be held: up to the first one without a page."""
+    t = 0
+    while t < want and (first + t) // page < table.shape[1] and named(table, s, (first + t) // page, pages):
+        t += 1
+    return t
+
+
 def attend(q, kv, table, lens, scale=None):
     """q [S, Hq, Dh] -> out [S, Hq, Dh], lse [S, Hq], given[s][h] [n] (the weight each held token gets), and
     spread [S, Hq, Dh] = sum_j p_j |v_j|, what errors of the weights are measured against."""
@@ -52,37 +65,40 @@ def add_given(weights, table, given, page):
 
 def append(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, w_new=None):
     S, H, T, _ = k_new.shape
-    page = kv.shape[3]
-    cap = table.shape[1] * page
+    pages, page = kv.shape[1], kv.shape[3]
     for s in range(S):
         n = T if n_new is None else int(n_new[s])
         for h in range(H):
-            for t in range(n):
+            take = with_a_page(table, s, int(lens[s, h]), n, page, pages)
+            for t in range(take):
                 i = int(lens[s, h]) + t
-                if i >= cap:
-                    break
                 pg, r = slot(table, s, i, page)
                 kv[0, pg, h, r], kv[1, pg, h, r] = k_new[s, h, t], v_new[s, h, t]
                 weights[pg, h, r] = 0.0 if w_new is None else w_new[s, h, t]
                 positions[pg, h, r] = next_pos[s, h] + t
-            lens[s, h] = min(lens[s, h] + n, cap)
+            lens[s, h] += take
             next_pos[s, h] += n
 
 
 def append_evict(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positions, keep, sink, recent, w_new=None):
     S, H, T, _ = k_new.shape
-    page = kv.shape[3]
+    pages, page = kv.shape[1], kv.shape[3]
     for s in range(S):
-        n = T if n_new is None else int(n_new[s])
         for h in range(H):
-            held = int(lens[s, h])
+            n = T if n_new is None else int(n_new[s])
+            held, end = int(lens[s, h]), int(next_pos[s, h]) + n
+            below = max(0, min(n, keep - held))                  # new tokens whose slot lies below the budget
+            if with_a_page(table, s, held, below, page, pages) < below:
+                n = with_a_page(table, s, held, below, page, pages)
             where = [slot(table, s, i, page) for i in range(held)]
-            rows = [(kv[0, a, h, r].copy(), kv[1, a, h, r].copy(), weights[a, h, r], int(positions[a, h, r])) for a, r in where]
+            rows = [(kv[0, a, h, r].copy(), kv[1, a, h, r].copy(), weights[a, h, r], int(positions[a, h, r]))
+                    if 0 <= a < pages else None for a, r in where]
             rows += [(k_new[s, h, t], v_new[s, h, t], 0.0 if w_new is None else w_new[s, h, t], int(next_pos[s, h]) + t)
                      for t in range(n)]
-            end = int(next_pos[s, h]) + n
 
             def order(i):
+                if i < held and rows[i] is None:   # a slot without a page: it can neither move nor be filled
+                    return (-1 if i < keep else 2, False, 0.0, i)
                 w, pos = rows[i][2], rows[i][3]
                 return (not (pos < sink or pos >= end - recent), not np.isnan(w), 0.0 if np.isnan(w) else -w, i)
             kept = sorted(range(len(rows)), key=order)[:keep]

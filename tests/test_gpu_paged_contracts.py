@@ -1,0 +1,115 @@
+"""What the paged cache promises about calls that go wrong or sit out: tokens and slots without a page."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_oracle
+from tests.paged_helpers import Cache, check_attention
+from world_engine_b200 import PagedSlab, ops
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(autouse=True)
+def healthy():
+    yield
+    ops.check_status(torch.device("cuda"))
+
+
+def reported():
+    with pytest.raises(RuntimeError, match="page"):
+        ops.check_status(torch.device("cuda"))
+
+
+def queries(c, G, seed=1):
+    g = torch.Generator().manual_seed(1000 + seed)
+    return torch.randn(c.S, c.H * G, 1, c.Dh, generator=g).to(c.dtype).cuda()
+
+
+def unname(c, *blocks):
+    """Takes pages out of the table: (session, block, what stands there instead)."""
+    for s, b, x in blocks:
+        c.table_h[s, b] = x
+    c.table.copy_(c.table_h)
+
+
+# ------------------------------------------------------------------------------------------------ tokens without a page
+@pytest.mark.parametrize("keep", [None, 96])
+def test_a_dropped_token_is_not_held(keep):
+    S, H, Dh, page = 3, 2, 64, 16
+    slab = PagedSlab(S, H, Dh, BF16, page, 20, 96, **({} if keep is None else dict(keep=keep, sink=2, recent=8)))
+    c = Cache(S, H, Dh, page, 6, BF16, lens=[0, 0, 0])
+    c.kv, c.weights, c.positions = slab.kv, slab.weights, slab.positions
+    c.table, c.lens, c.next_pos = slab.table, slab.lens, slab.next_pos
+    slab.kv.fill_(float("nan"))                  # what a page holds before its tokens are written
+    c.kv64, c.w64, c.pos64 = (x.cpu().numpy().copy() for x in (slab.kv.double(), slab.weights.double(), slab.positions))
+    c.lens64, c.next64 = np.zeros((S, H), np.int32), np.zeros((S, H), np.int32)
+
+    def step(T, seed):
+        (k, v, _), (k64, v64, _) = c.new(T, seed=seed)
+        slab.append(k, v)
+        c.table64 = slab.table.cpu().numpy()
+        if keep is None:
+            paged_oracle.append(c.kv64, c.table64, c.lens64, c.next64, k64, v64, None, c.w64, c.pos64)
+        else:
+            paged_oracle.append_evict(c.kv64, c.table64, c.lens64, c.next64, k64, v64, None, c.w64, c.pos64, keep, 2, 8)
+        c.assert_same_state()
+        q = queries(c, 2, seed)
+        before = c.w64.copy()
+        out = slab.attend(q)
+        check_attention(c, q, out, None, before, None if keep is None else slab.weights)
+        c.w64 = slab.weights.double().cpu().numpy()
+        return out
+
+    slab.reserve(0, 20)                          # 32 slots
+    slab.reserve(1, 16)
+    out = step(40, 1)
+    reported()
+    assert c.lens64.tolist() == [[32, 32], [16, 16], [0, 0]] and torch.all(out[2] == 0)
+    slab.reserve(0, 64)
+    slab.reserve(2, 3)
+    step(5, 2)
+    reported()                                   # (session 1 has no more room)
+    assert c.lens64.tolist() == [[37, 37], [16, 16], [5, 5]]
+    slab.reserve(1, 17)
+    step(1, 3)
+    assert c.lens64.tolist() == [[38, 38], [17, 17], [6, 6]]
+
+
+@pytest.mark.parametrize("T", [1, 7, 60, 900])
+@pytest.mark.parametrize("budget", [None, (1000, 3, 40)])
+@pytest.mark.parametrize("Dh,page,H", [(64, 16, 2), (128, 32, 1)])
+def test_counts_stop_at_the_first_token_without_a_page(T, budget, Dh, page, H):
+    lens = [0, page, 2 * page + 3, 5, page - 1, 10 * page, 3]
+    c = Cache(len(lens), H, Dh, page, -(-1300 // page), BF16, seed=T, lens=lens)
+    P = c.kv.shape[1]
+    # missing: the first page, the next one, the one it is in the middle of, a later one, one far away, none, the table's bound
+    unname(c, (0, 0, -1), (1, 1, P), (2, 2, -1), (3, 2, 2 ** 31 - 1), (4, 1, -1), (4, 2, -1), (6, 30, -2 ** 31))
+    (k, v, w), (k64, v64, w64) = c.new(T, seed=5, with_weights=True)
+    before = c.lens64.copy()
+    if budget is None:
+        ops.paged_append_(c.kv, c.table, c.lens, c.next_pos, k, v, None, c.weights, c.positions, w)
+        paged_oracle.append(c.kv64, c.table64, c.lens64, c.next64, k64, v64, None, c.w64, c.pos64, w64)
+    else:
+        ops.paged_append_evict_(c.kv, c.table, c.lens, c.next_pos, k, v, c.weights, c.positions, *budget, w_new=w)
+        paged_oracle.append_evict(c.kv64, c.table64, c.lens64, c.next64, k64, v64, None, c.w64, c.pos64, *budget, w64)
+    c.assert_same_state()
+    reported()
+    took = c.lens64 - before
+    assert np.all(took[0] == 0) and np.all(took[1] == 0) and np.all(took[2] == 0) and np.all(took[5] == min(T, 1000 - 10 * page if budget else T))
+    assert np.all(took[3] == min(T, 2 * page - 5)) and np.all(took[4] == 1)
+
+
+def test_a_long_append_stops_where_its_pages_do():
+    # more pages than one look of the CTA at the table; clusters of CTAs
+    for at in (0, 31, 32, 257, 1200):
+        c = Cache(1, 1, 64, 16, 1250, F16, seed=at, lens=[9])
+        unname(c, (0, at, -1), (0, at + 7, -1))
+        (k, v, _), (k64, v64, _) = c.new(19900, seed=6)
+        ops.paged_append_(c.kv, c.table, c.lens, c.next_pos, k, v, weights=c.weights, positions=c.positions)
+        paged_oracle.append(c.kv64, c.table64, c.lens64, c.next64, k64, v64, None, c.w64, c.pos64)
+        c.assert_same_state()
+        reported()
+        assert int(c.lens64[0, 0]) == max(16 * at, 9)

@@ -78,6 +78,33 @@ __device__ __forceinline__ float new_weight(const PagedAppendParams& p, int s, i
   return p.w_new != nullptr ? p.w_new[s * p.wns[0] + h * p.wns[1] + t * p.wns[2]] : 0.f;
 }
 
+// How many of `want` tokens from slot `first` on (all of them within the table) can be held: up to the first one for which
+// the table names no page.  Called by all threads of the CTA, with the same arguments; so is the answer.  Up to 32 pages
+// are looked up by every warp for itself, one load; more by the CTA together.
+__device__ __forceinline__ int with_a_page(const PagedView& v, int s, int first, int want, int* s_first_bad) {
+  if (want <= 0) return 0;
+  const int32_t* row = v.table + s * v.table_stride;
+  const int b0 = first >> v.page_shift, b1 = (first + want - 1) >> v.page_shift, lane = threadIdx.x & 31;
+  int bad = 0x7FFFFFFF;
+  if (b1 - b0 < 32) {
+    const int pg = b0 + lane <= b1 ? row[b0 + lane] : 0;
+    const uint32_t none = __ballot_sync(0xffffffffu, pg < 0 || pg >= v.n_pages);
+    if (none != 0) bad = b0 + __ffs(none) - 1;
+  } else {
+#pragma unroll 4
+    for (int b = b0 + static_cast<int>(threadIdx.x); b <= b1; b += static_cast<int>(blockDim.x)) {
+      const int pg = row[b];
+      if (pg < 0 || pg >= v.n_pages) bad = min(bad, b);
+    }
+    bad = __reduce_min_sync(0xffffffffu, bad);
+    if (lane == 0) s_first_bad[threadIdx.x >> 5] = bad;
+    __syncthreads();
+    const int warps = static_cast<int>(blockDim.x) >> 5;
+    bad = __reduce_min_sync(0xffffffffu, lane < warps ? s_first_bad[lane] : 0x7FFFFFFF);
+  }
+  return bad > b1 ? want : max((bad << v.page_shift) - first, 0);
+}
+
 // `items` moves of a token, one 16-byte vector of its K and of its V row per thread and step, kDepth steps at a time.
 // where(e, &src, &dst): src >= len is the new token src - len, anything else a slot.
 template <int kDepth, class F>
@@ -151,7 +178,9 @@ __global__ void __launch_bounds__(kAppendThreads, 6) paged_append_kernel(const P
   const int pos0 = p.next_pos[unit];
   const int n = new_count(p, s);
   const int room = (p.v.max_pages << p.v.page_shift) - len;
-  const int take = n < room ? n : room;
+  __shared__ int s_first_bad[kAppendThreads / 32];
+  // (a token that is dropped is not held: the count ends where the pages do)
+  const int take = with_a_page(p.v, s, len, n < room ? n : room, s_first_bad);
   if (take < n && threadIdx.x == 0) paged_report(p.v);
   const int32_t* table = p.v.table + s * p.v.table_stride;
   const int c = threadIdx.x & ((1 << p.vec_shift) - 1);
@@ -179,11 +208,7 @@ __global__ void __launch_bounds__(kAppendThreads, 6) paged_append_kernel(const P
 #pragma unroll
     for (int d = 0; d < kRows; ++d) {
       const int t = t0 + step * d, row = (len + t) & (p.v.page - 1);
-      if (t >= take) continue;
-      if (pg[d] < 0 || pg[d] >= p.v.n_pages) {
-        paged_report(p.v);
-        continue;
-      }
+      if (t >= take || static_cast<uint32_t>(pg[d]) >= static_cast<uint32_t>(p.v.n_pages)) continue;   // (looked up twice)
       uint16_t* dst = kv + pg[d] * p.v.page_s + row * p.v.token_s;
       *reinterpret_cast<uint4*>(dst) = k[d];
       *reinterpret_cast<uint4*>(dst + p.v.plane_s) = v[d];
@@ -275,17 +300,28 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) paged_appen
   for (int b = tid; b < digits.passes * bins / 4; b += kThreads) reinterpret_cast<uint4*>(s_hist)[b] = make_uint4(0u, 0u, 0u, 0u);
   // One CTA starts at the first token whatever the counts are: its pages are looked up while they are on their way.
   int early[kGroups];
+  auto look_up = [&]() {
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
-    const int b = (4 * (g * kThreads + tid)) >> p.v.page_shift;
-    early[g] = p.cluster == 1 && b < p.v.max_pages ? p.v.table[s * p.v.table_stride + b] : 0;
-  }
+    for (int g = 0; g < kGroups; ++g) {
+      const int b = (4 * (g * kThreads + tid)) >> p.v.page_shift;
+      early[g] = p.cluster == 1 && b < p.v.max_pages ? p.v.table[s * p.v.table_stride + b] : 0;
+    }
+  };
+  look_up();
   const int len = paged_count(p.v, p.lens[unit]);
   const int pos0 = p.next_pos[unit];
-  const int n = new_count(p, s);
-  const int total = len + n;
+  int n = new_count(p, s);
   const int64_t end = static_cast<int64_t>(pos0) + n;
   __syncthreads();
+  if (len < p.keep) {                                    // below the budget a token goes to the next slot, if it has a page
+    const int have = with_a_page(p.v, s, len, min(n, p.keep - len), reinterpret_cast<int*>(s_warp));
+    if (have < min(n, p.keep - len)) {                   // the rest is dropped
+      n = have;
+      if (tid == 0) paged_report(p.v);
+    }
+    look_up();                                           // (again: a session at its budget comes past here, in registers)
+  }
+  const int total = len + n;
   if (total <= p.keep) {
     move_tokens<2>(p, s, h, len, pos0, n, rank * kThreads + tid, p.cluster * kThreads,
                    [&](int e, int* src, int* dst) { *src = *dst = len + e; });

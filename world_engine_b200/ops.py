@@ -401,7 +401,8 @@ def paged_append_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, nex
     `table [S, M]` the pages of session s, `lens` / `next_pos` `[S, Hkv]` the tokens a kv head holds and was ever
     given.  `k_new` / `v_new` are `[S, Hkv, T, Dh]` views (any strides, head dim contiguous); of a padded batch only
     the first `n_new[s]` tokens count.  The counts are updated in place unless `lens_out` / `next_pos_out` are
-    given.  Tokens for which a session has no room are dropped and reported by `check_status`."""
+    given.  The first token for which a session has no page is dropped with all behind it and reported by
+    `check_status`: `lens` counts what is held, `next_pos` what was given."""
     _append(_lib.load().we_b200_paged_append, "we_b200_paged_append", kv, table, lens, next_pos, k_new, v_new, n_new,
             weights, positions, w_new, lens_out, next_pos_out, 0, 0, 0)
 

@@ -14,7 +14,8 @@ never change and its steps can be captured in a CUDA graph.
 
 The host never reads the device: pages are handed out by `reserve`, which the
 caller asks for what a session is going to hold.  A token for which its session
-has no page is dropped and reported by `ops.check_status`.
+has no page is dropped, with those behind it, and reported by `ops.check_status`:
+`lens` counts what is held, so a session can go on after a later `reserve`.
 """
 from __future__ import annotations
 
