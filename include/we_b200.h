@@ -339,8 +339,13 @@ WE_B200_API int we_b200_paged_append(const we_b200_paged_append_args* args_host,
  * evicted ones left, both in ascending order; the others stay where they are,
  * so little is moved.  What an evicted slot beyond the budget holds is left as
  * it was.  A token whose slot would lie below the budget is dropped where the
- * table names no page for it, as above.  The workspace (we_b200_paged_evict_workspace_bytes) needs no
- * initialisation.  max_pages * page + T < 2^21.
+ * table names no page for it, as above.  Of slots that count as held although
+ * the table names no page for them, those below the budget stay held, with
+ * nothing moved there (as many fewer tokens find room), the others are given up.
+ * The positions of a kv head's tokens are distinct, as appends make them, so at
+ * most `keep` are shielded (of more, the lowest indexes would stay).
+ * The workspace (we_b200_paged_evict_workspace_bytes) needs no initialisation.
+ * max_pages * page + T < 2^21.
  */
 WE_B200_API int we_b200_paged_append_evict(const we_b200_paged_append_args* args_host, int32_t* status, void* stream);
 WE_B200_API size_t we_b200_paged_evict_workspace_bytes(const we_b200_paged_geom* geom_host, int32_t T, int32_t keep);

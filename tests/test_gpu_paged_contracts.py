@@ -113,3 +113,46 @@ def test_a_long_append_stops_where_its_pages_do():
         c.assert_same_state()
         reported()
         assert int(c.lens64[0, 0]) == max(16 * at, 9)
+
+
+# ------------------------------------------------------------------------------------------------ held slots without a page
+@pytest.mark.parametrize("lens,T,keep,sink,recent,blocks", [
+    ([64, 64], 3, 64, 2, 20, [(0, 1)]),                  # at the budget
+    ([64, 60], 1, 64, 2, 62, [(0, 0), (1, 2)]),          # all the rest is shielded: the newest of them go without a slot
+    ([90, 70], 3, 50, 1, 30, [(0, 1), (0, 4), (1, 3)]),  # the budget was lowered: slots of either side
+    ([90, 70], 0, 20, 0, 0, [(0, 2), (0, 3), (0, 4), (0, 5), (1, 0)]),
+    ([48, 64], 200, 64, 4, 16, [(0, 0), (1, 3)]),        # a prompt
+    ([64, 64], 5, 64, 0, 0, [(0, 0), (0, 1), (0, 2), (0, 3)])])   # no page at all
+@pytest.mark.parametrize("with_weights", [False, True])
+def test_eviction_neither_keeps_nor_fills_a_slot_without_a_page(lens, T, keep, sink, recent, blocks, with_weights):
+    c = Cache(2, 2, 64, 16, 6, BF16, seed=T + keep, lens=lens)
+    for s in range(2):                                   # odd weights among them: the last word must not be theirs
+        c.weights[c.table[s, 0].long(), 0, 3] = float("inf")
+        c.weights[c.table[s, 0].long(), 0, 5] = float("nan")
+        c.weights[c.table[s, 0].long(), 1, 3] = float("-inf")
+    c.w64 = c.weights.double().cpu().numpy()
+    unname(c, *((s, b, -1) for s, b in blocks))
+    (k, v, w), (k64, v64, w64) = c.new(T, seed=7, with_weights=with_weights)
+    ops.paged_append_evict_(c.kv, c.table, c.lens, c.next_pos, k, v, c.weights, c.positions, keep, sink, recent, w_new=w)
+    paged_oracle.append_evict(c.kv64, c.table64, c.lens64, c.next64, k64, v64, None, c.w64, c.pos64, keep, sink, recent, w64)
+    c.assert_same_state()
+    reported()
+
+
+@pytest.mark.parametrize("H,idle,held,keep,T", [(1, 0, 20000, 20000, 50), (3, 120, 5400, 5300, 9), (2, 0, 40000, 33333, 17)])
+def test_long_evictions_around_slots_without_a_page(H, idle, held, keep, T):
+    # clusters; CTAs that go through their candidates in rounds (beside sessions that hold nothing)
+    c = Cache(2, H, 64, 64, -(-held // 64), F16, seed=H, lens=[held, held - 1])
+    unname(c, (0, 0, -1), (0, 50, -1), (0, held // 64 - 1, c.kv.shape[1]), (1, keep // 64, -1))
+    (k, v, w), (k64, v64, w64) = c.new(T, seed=8, with_weights=True)
+
+    def padded(x, value=0):
+        return torch.cat([x, torch.full((idle, *x.shape[1:]), value, dtype=x.dtype, device="cuda")])
+    table, lens, next_pos = padded(c.table, -1), padded(c.lens), padded(c.next_pos)
+    n_new = torch.tensor([T, T] + [0] * idle, dtype=torch.int32, device="cuda")
+    ops.paged_append_evict_(c.kv, table, lens, next_pos, padded(k), padded(v), c.weights, c.positions, keep, 4, 100, n_new, padded(w))
+    assert not lens[2:].any() and not next_pos[2:].any()
+    c.lens, c.next_pos = lens[:2], next_pos[:2]
+    paged_oracle.append_evict(c.kv64, c.table64, c.lens64, c.next64, k64, v64, None, c.w64, c.pos64, keep, 4, 100, w64)
+    c.assert_same_state()
+    reported()

@@ -230,8 +230,13 @@ __global__ void __launch_bounds__(kAppendThreads, 6) paged_append_kernel(const P
 
 // ------------------------------------------------------------------ under a budget
 // Weights as unsigned numbers of the same order: NaN above every number, shielded tokens above NaN, -0 equal to 0.
+// A held slot for which the table names no page holds nothing that could be kept or moved, and nothing can be put there.
+// Below the budget it stays where it is, above everything (it can be neither a hole nor a mover, and the tokens with the
+// least weight go for want of a slot); behind the budget it comes below everything, and is given up: there are always
+// `keep` others, as all indexes below the budget are candidates.
+constexpr uint32_t kKeyNan = 0xFFFFFFFDu, kKeyShielded = 0xFFFFFFFEu, kKeyFixed = 0xFFFFFFFFu, kKeyNothing = 0u;
 __device__ __forceinline__ uint32_t weight_key(float w) {
-  if (w != w) return 0xFFFFFFFEu;
+  if (w != w) return kKeyNan;
   const uint32_t b = __float_as_uint(w == 0.f ? 0.f : w);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
@@ -332,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) paged_appen
     const int rounds = (mine + kRound - 1) / kRound;
     const bool fits = slice <= p.fit;
     auto key_of = [&](float w, int64_t pos) {
-      return pos < p.sink || pos >= end - p.recent ? 0xFFFFFFFFu : weight_key(w);
+      return pos < p.sink || pos >= end - p.recent ? kKeyShielded : weight_key(w);
     };
     uint32_t key[kGroups][4];                            // (those behind the slice: unused)
     auto first_of = [&](int round, int g) { return lo + round * kRound + 4 * (g * kThreads + tid); };
@@ -354,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) paged_appen
           w[b] = make_float4(0.f, 0.f, 0.f, 0.f);
           pos[b] = make_int4(0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF, 0x7FFFFFFF);
           if (i >= hi || i >= len) continue;
-          if (pg[g] < 0 || pg[g] >= p.v.n_pages) {       // taken for tokens nobody looked at
+          if (pg[g] < 0 || pg[g] >= p.v.n_pages) {
             paged_report(p.v);
             continue;
           }
@@ -370,6 +375,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 1) paged_appen
           key[g][1] = key_of(w[b].y, pos[b].y);
           key[g][2] = key_of(w[b].z, pos[b].z);
           key[g][3] = key_of(w[b].w, pos[b].w);
+          if (i < len && (pg[g] < 0 || pg[g] >= p.v.n_pages)) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) key[g][u] = i + u < p.keep ? kKeyFixed : kKeyNothing;
+          }
           if (i + 3 < len) continue;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
