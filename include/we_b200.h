@@ -45,7 +45,7 @@
 extern "C" {
 #endif
 
-#define WE_B200_ABI_VERSION 1
+#define WE_B200_ABI_VERSION 2
 
 #if defined(__GNUC__)
 #define WE_B200_API __attribute__((visibility("default")))
@@ -364,6 +364,7 @@ typedef struct we_b200_paged_attn_args {
   uint64_t workspace_bytes;
   int32_t Hq;
   float scale;                  /* <= 0: 1/sqrt(Dh)                                 */
+  const int32_t* n_new;         /* [S]: sessions with n_new[s] < 1 sit out; or NULL */
 } we_b200_paged_attn_args;
 
 /*
@@ -372,12 +373,16 @@ typedef struct we_b200_paged_attn_args {
  * for every query head g of kv head h = g / (Hq / Hkv).  With `weights`, the
  * token j of kv head h has sum_g p_gj added to its weight; with `lse`, the
  * logarithm of the softmax sum (natural units) is stored.  A head that holds
- * nothing gives 0 and -inf.  Workspace: we_b200_paged_attn_workspace_bytes,
- * contents irrelevant before and after.  out must not overlap q.
+ * nothing gives 0 and -inf.  So does a session that sits out (n_new[s] < 1, as
+ * in a padded append): nothing of its cache or its q is read or given weight.
+ * Workspace: we_b200_paged_attn_workspace_bytes (`uses`: the sum of
+ * WE_B200_USES_... for what the call gives), contents irrelevant before and
+ * after.  out must not overlap q.
  */
+enum { WE_B200_USES_WEIGHTS = 1, WE_B200_USES_N_NEW = 2 };
 WE_B200_API int we_b200_paged_attn(const we_b200_paged_attn_args* args_host, int32_t* status, void* stream);
 WE_B200_API size_t we_b200_paged_attn_workspace_bytes(const we_b200_paged_geom* geom_host, int32_t Hq,
-                                                      int accumulate);
+                                                      int uses);
 
 /* Number of kernels the previous three entry points have launched in this
  * process (diagnostic counter for benchmarks; relaxed atomics). */

@@ -1,4 +1,5 @@
-"""What the paged cache promises about calls that go wrong or sit out: tokens and slots without a page."""
+"""What the paged cache promises about calls that go wrong or sit out: tokens without a page, sessions without a new token,
+the ends of the number range, reports across graph replays."""
 import numpy as np
 import pytest
 import torch
@@ -156,3 +157,73 @@ def test_long_evictions_around_slots_without_a_page(H, idle, held, keep, T):
     paged_oracle.append_evict(c.kv64, c.table64, c.lens64, c.next64, k64, v64, None, c.w64, c.pos64, keep, 4, 100, w64)
     c.assert_same_state()
     reported()
+
+
+# ------------------------------------------------------------------------------------------------ sessions that sit out
+@pytest.mark.parametrize("S,H,G,page,M,most", [
+    (6, 2, 1, 16, 8, 128),            # never split
+    (6, 2, 4, 16, 40, 640),           # split and joined
+    (14, 5, 20, 16, 512, 8192),       # runs handed out, two units per kv head
+    (140, 3, 2, 32, 6, 190)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_a_session_that_sits_out_is_left_alone(S, H, G, page, M, most, accumulate):
+    lens = [[(most * (1 + (7 * s + 3 * h) % 11)) // 11 if most < 1000 else most - 13 * s - h for h in range(H)] for s in range(S)]
+    c = Cache(S, H, 64, page, M, BF16, seed=S, lens=lens)
+    q = queries(c, G)
+    out_of_step = [s for s in range(S) if s % 3 == 1]
+    q[out_of_step] = float("nan")                        # rows of a padded batch
+    n_new = torch.ones(S, dtype=torch.int32, device="cuda")
+    n_new[out_of_step] = 0
+    n_new[out_of_step[-1]] = -1
+    n_new[0] = 7
+    weights = c.weights if accumulate else None
+    lse = torch.zeros(S, H * G, device="cuda")
+    out = ops.paged_attn(q, c.kv, c.table, c.lens, weights=weights, lse=lse, n_new=n_new)
+    assert torch.all(out[out_of_step] == 0) and torch.all(torch.isneginf(lse[out_of_step]))
+    before = c.w64.copy()
+    c.lens64[out_of_step] = 0                            # as if they held nothing
+    check_attention(c, torch.where(n_new[:, None, None, None] > 0, q, 0.0), out, lse, before, weights)
+    if accumulate:
+        pages = c.table[out_of_step].long().flatten()
+        assert torch.equal(c.weights[pages].double().cpu().nan_to_num(7.0), torch.from_numpy(before)[pages.cpu()].nan_to_num(7.0))
+    held = c.lens.clone()
+    held[out_of_step] = 0
+    c.weights.copy_(torch.from_numpy(before).float())
+    assert torch.equal(out, ops.paged_attn(q, c.kv, c.table, held, weights=weights))
+
+
+@pytest.mark.parametrize("budget", [dict(), dict(keep=20, sink=1, recent=4)])
+@pytest.mark.parametrize("compiled", [False, True])
+def test_a_step_that_some_sessions_sit_out(budget, compiled):
+    """A padded step leaves the sessions that sit out as they were, and the others as steps without them do."""
+    def slab():
+        x = PagedSlab(3, 2, 64, BF16, 16, 12, 48, **budget)
+        for s in range(3):
+            x.reserve(s, 20 if budget else 48)
+        return x
+    every, alone = slab(), [PagedSlab(1, 2, 64, BF16, 16, 4, 48, **budget) for _ in range(3)]
+    for x in alone:
+        x.reserve(0, 20 if budget else 48)
+    g = torch.Generator().manual_seed(2)
+    step = every.append_and_attend
+    if compiled:
+        step = torch.compile(lambda q, k, v, n: every.append_and_attend(q, k, v, n), fullgraph=True, backend="aot_eager")
+    for i in range(30):
+        q, k, v = (torch.randn(3, n, 1, 64, generator=g).to(BF16).cuda() for n in (4, 2, 2))
+        n_new = torch.tensor([1, i % 2, i % 3 != 0], dtype=torch.int32)
+        idle = [s for s in range(3) if n_new[s] == 0]
+        for x in (q, k, v):
+            x[idle] = float("nan")
+        with torch.no_grad():
+            y = step(q, k, v, n_new.cuda())
+        for s in range(3):
+            if s in idle:
+                assert torch.all(y[s] == 0)
+            else:
+                z = alone[s].append_and_attend(q[s:s + 1], k[s:s + 1], v[s:s + 1]).float()
+                # (cut into other runs: the sums are added up in another order)
+                assert torch.allclose(y[s].float(), z[0], rtol=2 ** -6, atol=2 ** -10)
+    for s in range(3):
+        assert torch.equal(every.lens[s], alone[s].lens[0]) and torch.equal(every.next_pos[s], alone[s].next_pos[0])
+        assert torch.isfinite(every.weights).all()
+    assert every.next_pos[:, 0].tolist() == [30, 15, 20]

@@ -1,0 +1,38 @@
+"""What the paged cache promises where no GPU is needed: refusals, sizes of workspaces."""
+import ctypes
+
+import pytest
+import torch
+
+from tests.test_paged_refusals import FAKE, attn_args, attn_metas, geom, meta
+from world_engine_b200 import _lib, ops
+from world_engine_b200.csrc import build as csrc_build
+
+
+@pytest.fixture(scope="module")
+def lib():
+    csrc_build.build()
+    return _lib.load()
+
+
+def test_who_sits_out_is_checked(lib):
+    good = meta((3,), torch.int32)
+    plain, padded = ops._attn_plan(**attn_metas()), ops._attn_plan(**attn_metas(), n_new=good)
+    assert padded[:2] == plain[:2] and padded[2] == plain[2] + 3 * 4 * 4
+    for bad in (meta((3,), torch.int64), meta((4,), torch.int32), meta((3, 1), torch.int32), meta((3,), torch.int32, stride=(2,)),
+                meta((3,), torch.int32, device=1)):
+        with pytest.raises(ValueError):
+            ops._attn_plan(**attn_metas(), n_new=bad)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops._attn_plan(**attn_metas(), n_new=meta((3,), torch.int32, device=-1))
+
+
+@pytest.mark.parametrize("max_pages", [4, 400])
+@pytest.mark.parametrize("weights", [0, 1])
+def test_sitting_out_needs_a_workspace(lib, max_pages, weights):
+    g = geom(max_pages=max_pages, table_stride=max_pages)
+    need = lib.we_b200_paged_attn_workspace_bytes(ctypes.byref(g), 8, weights)
+    more = lib.we_b200_paged_attn_workspace_bytes(ctypes.byref(g), 8, weights + 2)
+    assert more == need + 3 * 4 * 4 and (need == 0) == (max_pages == 4 and not weights)
+    a = attn_args(g, n_new=FAKE, weights=FAKE if weights else None, workspace_bytes=more - 1)
+    assert lib.we_b200_paged_attn(ctypes.byref(a), None, None) == -5

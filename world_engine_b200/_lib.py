@@ -12,7 +12,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libwe_b200.so"
-ABI_VERSION = 1
+ABI_VERSION = 2
 
 BF16, F16, F32 = 0, 1, 2
 
@@ -100,7 +100,7 @@ class PagedAttnArgs(ctypes.Structure):
         ("q", c_void_p), ("out", c_void_p), ("q_strides", Strides2), ("out_strides", Strides2),
         ("kv", c_void_p), ("table", c_void_p), ("lens", c_void_p), ("weights", c_void_p), ("lse", c_void_p),
         ("workspace", c_void_p), ("workspace_bytes", c_uint64),
-        ("Hq", c_int32), ("scale", c_float),
+        ("Hq", c_int32), ("scale", c_float), ("n_new", c_void_p),
     ]
 
 
@@ -108,7 +108,7 @@ class PagedAttnArgs(ctypes.Structure):
 # microseconds to fill field by field).
 _GEOM_FORMAT = "8i5q"
 PAGED_APPEND_PACK = struct.Struct("=" + _GEOM_FORMAT + "2Q6q10Q3q2Q4i")
-PAGED_ATTN_PACK = struct.Struct("=" + _GEOM_FORMAT + "2Q4q7Qif")
+PAGED_ATTN_PACK = struct.Struct("=" + _GEOM_FORMAT + "2Q4q7QifQ")
 assert PAGED_APPEND_PACK.size == ctypes.sizeof(PagedAppendArgs)
 assert PAGED_ATTN_PACK.size == ctypes.sizeof(PagedAttnArgs)
 

@@ -307,6 +307,11 @@ def _check_paged(kv, table, counts, per_slot, others) -> Tuple[int, ...]:
     return (S, Hkv, Dh, page, P, M, dtype_code(dtype), 0, stride[0], stride[1], stride[2], stride[3], table[1][0])
 
 
+def _check_n_new(meta, S: int) -> None:
+    if meta != _NONE and (meta[2] != torch.int32 or meta[0] != (S,) or not _dense(meta)):
+        raise ValueError("n_new must be contiguous int32 [S]")
+
+
 def _dense(meta) -> bool:
     want = 1
     for n, s in zip(reversed(meta[0]), reversed(meta[1])):
@@ -352,8 +357,7 @@ def _append_plan(kv, table, lens, next_pos, lens_out, next_pos_out, k_new, v_new
     if len(shape) != 4 or (shape[0], shape[1], shape[3]) != (S, Hkv, Dh) or v_new[0] != shape \
             or k_new[2] != kv[2] or v_new[2] != kv[2] or k_new[1][3] != 1 or v_new[1][3] != 1:
         raise ValueError("k_new and v_new must be [S, Hkv, T, Dh] of the cache's type with a contiguous last axis")
-    if n_new != _NONE and (n_new[2] != torch.int32 or n_new[0] != (S,) or not _dense(n_new)):
-        raise ValueError("n_new must be contiguous int32 [S]")
+    _check_n_new(n_new, S)
     if w_new != _NONE and (w_new[2] != torch.float32 or w_new[0] != shape[:3]):
         raise ValueError("w_new must be float32 [S, Hkv, T]")
     need = 0
@@ -424,9 +428,9 @@ def paged_append_evict_(kv: torch.Tensor, table: torch.Tensor, lens: torch.Tenso
             v_new, n_new, weights, positions, w_new, lens_out, next_pos_out, keep, sink, recent)
 
 
-def _attn_plan(q, kv, table, lens, weights, out, lse):
-    """Checks of an attention call; (geometry, workspace bytes)."""
-    geom = _check_paged(kv, table, (lens,), (weights,), (q, out, lse))
+def _attn_plan(q, kv, table, lens, weights, out, lse, n_new=_NONE):
+    """Checks of an attention call; (geometry, shape, workspace bytes)."""
+    geom = _check_paged(kv, table, (lens,), (weights,), (q, out, lse, n_new))
     S, _, Dh = geom[:3]
     shape = q[0]
     if len(shape) != 4 or (shape[0], shape[2], shape[3]) != (S, 1, Dh) or q[2] != kv[2] or q[1][3] != 1:
@@ -435,18 +439,21 @@ def _attn_plan(q, kv, table, lens, weights, out, lse):
         raise ValueError("out must have q's shape and type and a contiguous last axis")
     if lse != _NONE and (lse[2] != torch.float32 or lse[0] != shape[:2] or not _dense(lse)):
         raise ValueError("lse must be contiguous float32 [S, Hq]")
-    need = _lib.load().we_b200_paged_attn_workspace_bytes(ctypes.byref(PagedGeom(*geom)), shape[1], weights != _NONE)
+    _check_n_new(n_new, S)
+    need = _lib.load().we_b200_paged_attn_workspace_bytes(
+        ctypes.byref(PagedGeom(*geom)), shape[1], (weights != _NONE) + 2 * (n_new != _NONE))
     return geom, (S, shape[1], 1, Dh), need
 
 
 def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float = 0.0,
                weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-               lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+               lse: Optional[torch.Tensor] = None, n_new: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one new token per session over its paged cache (we_b200_paged_attn).  `q` is a
     `[S, Hq, 1, Dh]` view; the output has its shape.  With `weights` the softmax weight every held token is given
     (summed over the query heads of its kv head) is added to it in place; `lse` (float32 `[S, Hq]`, contiguous)
-    receives the logarithm of the softmax sum.  A kv head that holds nothing gives 0 and -inf.  `out` must not overlap
-    `q`.  Results repeat bit for bit (but for the weights of pages that several sessions share)."""
+    receives the logarithm of the softmax sum.  A kv head that holds nothing gives 0 and -inf.  So does a
+    session that sits out (`n_new[s] < 1`, int32 `[S]`, as in a padded append): its weights stay as they are, and
+    neither its cache nor its row of `q` is read.  `out` must not overlap `q`.  Results repeat bit for bit (but for the weights of pages that several sessions share)."""
     if torch.is_grad_enabled():
         _refuse_grad(q, kv, weights, out, lse)
     index, qs = q.get_device(), q.stride()
@@ -456,7 +463,8 @@ def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: tor
            lens.shape, lens.stride(), lens.dtype, lens.get_device(),
            *(_NONE if weights is None else (weights.shape, weights.stride(), weights.dtype, weights.get_device())),
            *(_NONE if out is None else (out.shape, out.stride(), out.dtype, out.get_device())),
-           *(_NONE if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.get_device())))
+           *(_NONE if lse is None else (lse.shape, lse.stride(), lse.dtype, lse.get_device())),
+           *(_NONE if n_new is None else (n_new.shape, n_new.stride(), n_new.dtype, n_new.get_device())))
     geom, shape, need = _attn_plans.get(key) or _plan(_attn_plans, _attn_plan, key)
     if out is None:
         out = torch.empty_like(q)
@@ -467,7 +475,8 @@ def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: tor
     _call_paged(_lib.load().we_b200_paged_attn, _lib.PAGED_ATTN_PACK.pack(
         *geom, q.data_ptr(), out.data_ptr(), qs[0], qs[1], os_[0], os_[1], kv.data_ptr(), table.data_ptr(),
         lens.data_ptr(), 0 if weights is None else weights.data_ptr(), 0 if lse is None else lse.data_ptr(),
-        0 if ws is None else ws.data_ptr(), need, shape[1], scale), index, "we_b200_paged_attn")
+        0 if ws is None else ws.data_ptr(), need, shape[1], scale, 0 if n_new is None else n_new.data_ptr()),
+        index, "we_b200_paged_attn")
     return out
 
 
@@ -573,10 +582,10 @@ def _paged_append_evict_fake(kv, table, lens, next_pos, k_new, v_new, weights, p
 
 @torch.library.custom_op("world_engine_b200::paged_attn", mutates_args=("weights",))
 def paged_attn_op(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: float,
-                  weights: Optional[torch.Tensor]) -> torch.Tensor:
-    return paged_attn(q, kv, table, lens, scale, weights)
+                  weights: Optional[torch.Tensor], n_new: Optional[torch.Tensor] = None) -> torch.Tensor:
+    return paged_attn(q, kv, table, lens, scale, weights, n_new=n_new)
 
 
 @paged_attn_op.register_fake
-def _paged_attn_fake(q, kv, table, lens, scale, weights):
+def _paged_attn_fake(q, kv, table, lens, scale, weights, n_new=None):
     return q.new_empty(q.shape)

@@ -93,16 +93,18 @@ class PagedSlab:
             a = (self.kv, self.table, self.lens, self.next_pos, k, v, n_new, self.weights, self.positions, w_new)
             (ops.paged_append_op if torch.compiler.is_compiling() else ops.paged_append_)(*a)
 
-    def attend(self, q: Tensor, scale: float = 0.0) -> Tensor:
-        """q [S, Hq, 1, Dh] over what every session holds; under a budget the weights are added up."""
+    def attend(self, q: Tensor, scale: float = 0.0, n_new: Optional[Tensor] = None) -> Tensor:
+        """q [S, Hq, 1, Dh] over what every session holds; under a budget the weights are added up.  Sessions with
+        `n_new[s] == 0` sit out: their rows of the output are 0 and their weights stay as they are."""
         weights = self.weights if self.keep is not None else None
         if torch.compiler.is_compiling():
-            return ops.paged_attn_op(q, self.kv, self.table, self.lens, float(scale), weights)
-        return ops.paged_attn(q, self.kv, self.table, self.lens, float(scale), weights)
+            return ops.paged_attn_op(q, self.kv, self.table, self.lens, float(scale), weights, n_new)
+        return ops.paged_attn(q, self.kv, self.table, self.lens, float(scale), weights, n_new=n_new)
 
     def append_and_attend(self, q: Tensor, k: Tensor, v: Tensor, n_new: Optional[Tensor] = None,
                           scale: float = 0.0) -> Tensor:
         """One decoding step: append k / v [S, H, 1, Dh], then attend with q [S, Hq, 1, Dh].  Sessions with
-        `n_new[s] == 0` do not grow; one that holds nothing gets zeros."""
+        `n_new[s] == 0` sit the step out (their rows of q, k and v are not read): nothing of theirs changes, and their
+        rows of the output are 0."""
         self.append(k, v, n_new)
-        return self.attend(q, scale)
+        return self.attend(q, scale, n_new)
