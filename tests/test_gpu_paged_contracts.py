@@ -227,3 +227,18 @@ def test_a_step_that_some_sessions_sit_out(budget, compiled):
         assert torch.equal(every.lens[s], alone[s].lens[0]) and torch.equal(every.next_pos[s], alone[s].next_pos[0])
         assert torch.isfinite(every.weights).all()
     assert every.next_pos[:, 0].tolist() == [30, 15, 20]
+
+
+def test_traces_with_permuted_queries():
+    c = Cache(3, 2, 64, 16, 9, BF16, seed=4, lens=[100, 3, 144])
+    x = torch.randn(8, 3, 1, 64, device="cuda").to(BF16)
+
+    def step(x):
+        y = ops.paged_attn_op(x.transpose(0, 1), c.kv, c.table, c.lens, 0.0, None)
+        return y.transpose(0, 1).reshape(8, -1) + 1, y
+    with torch.no_grad():
+        flat, y = torch.compile(step, fullgraph=True, backend="aot_eager")(x)
+        want_flat, want = step(x)
+    assert torch.equal(y, want) and y.stride() == want.stride() and torch.equal(flat, want_flat)
+    q = x.transpose(0, 1)
+    check_attention(c, q, y)

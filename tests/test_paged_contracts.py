@@ -1,8 +1,9 @@
-"""What the paged cache promises where no GPU is needed: refusals, sizes of workspaces."""
+"""What the paged cache promises where no GPU is needed: refusals, sizes of workspaces, layouts under tracing."""
 import ctypes
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from tests.test_paged_refusals import FAKE, attn_args, attn_metas, geom, meta
 from world_engine_b200 import _lib, ops
@@ -36,3 +37,15 @@ def test_sitting_out_needs_a_workspace(lib, max_pages, weights):
     assert more == need + 3 * 4 * 4 and (need == 0) == (max_pages == 4 and not weights)
     a = attn_args(g, n_new=FAKE, weights=FAKE if weights else None, workspace_bytes=more - 1)
     assert lib.we_b200_paged_attn(ctypes.byref(a), None, None) == -5
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2, 3), (1, 0, 2, 3), (2, 1, 0, 3), (1, 2, 0, 3)])
+def test_a_traced_output_has_the_strides_of_the_real_one(order):
+    shape = (4, 8, 1, 64)
+    with FakeTensorMode():
+        q = torch.empty([shape[i] for i in order], dtype=torch.bfloat16).permute([order.index(i) for i in range(4)])
+        assert q.shape == shape
+        kv = torch.empty(2, 9, 2, 16, 64, dtype=torch.bfloat16)
+        table, lens = torch.empty(4, 2, dtype=torch.int32), torch.empty(4, 2, dtype=torch.int32)
+        out = ops.paged_attn_op(q, kv, table, lens, 0.0, None)
+        assert out.shape == shape and out.stride() == torch.empty_like(q).stride()

@@ -588,4 +588,4 @@ def paged_attn_op(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: 
 
 @paged_attn_op.register_fake
 def _paged_attn_fake(q, kv, table, lens, scale, weights, n_new=None):
-    return q.new_empty(q.shape)
+    return torch.empty_like(q)
