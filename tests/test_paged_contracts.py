@@ -3,10 +3,11 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from tests.test_paged_refusals import FAKE, attn_args, attn_metas, geom, meta
-from world_engine_b200 import _lib, ops
+from world_engine_b200 import PagedSlab, _lib, ops
 from world_engine_b200.csrc import build as csrc_build
 
 
@@ -49,3 +50,18 @@ def test_a_traced_output_has_the_strides_of_the_real_one(order):
         table, lens = torch.empty(4, 2, dtype=torch.int32), torch.empty(4, 2, dtype=torch.int32)
         out = ops.paged_attn_op(q, kv, table, lens, 0.0, None)
         assert out.shape == shape and out.stride() == torch.empty_like(q).stride()
+
+
+def test_ops_refuse_what_has_a_tangent():
+    slab = PagedSlab(2, 2, 64, torch.bfloat16, 16, 4, 32, keep=20, device="cpu")
+    x = torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16)
+    w = torch.zeros(2, 2, 1)
+    with forward_ad.dual_level():
+        d, dw = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: slab.append(d, x), lambda: slab.append(x, d), lambda: slab.append(x, x, w_new=dw), lambda: slab.attend(d)):
+            with pytest.raises(RuntimeError, match="derivative"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="derivative"):
+                call()
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            slab.append(x, x)

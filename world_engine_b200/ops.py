@@ -12,6 +12,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import CacheGeom, PagedGeom, PrologueArgs, Strides3
@@ -279,6 +280,13 @@ def _refuse_grad(*tensors) -> None:
             raise RuntimeError("the paged cache operators have no backward pass; call them under torch.no_grad()")
 
 
+def _refuse_tangents(*tensors) -> None:
+    """Within forward_ad.dual_level() (which torch.no_grad() does not end)."""
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the paged cache operators have no forward derivative; give them the primals")
+
+
 def _check_paged(kv, table, counts, per_slot, others) -> Tuple[int, ...]:
     """What every paged entry point checks; the geometry's fields.  A tensor is given as its (shape, strides, type,
     device index), one that is left out as `_NONE`."""
@@ -370,6 +378,8 @@ def _append(fn, where, kv, table, lens, next_pos, k_new, v_new, n_new, weights, 
             next_pos_out, keep, sink, recent) -> None:
     if torch.is_grad_enabled():
         _refuse_grad(kv, k_new, v_new, weights, w_new)
+    if getattr(_forward_ad, "_current_level", 0) >= 0:         # (-1: nobody is taking forward derivatives)
+        _refuse_tangents(kv, k_new, v_new, weights, w_new)
     index = kv.get_device()
     key = (kv.shape, kv.stride(), kv.dtype, index,
            table.shape, table.stride(), table.dtype, table.get_device(),
@@ -456,6 +466,8 @@ def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: tor
     neither its cache nor its row of `q` is read.  `out` must not overlap `q`.  Results repeat bit for bit (but for the weights of pages that several sessions share)."""
     if torch.is_grad_enabled():
         _refuse_grad(q, kv, weights, out, lse)
+    if getattr(_forward_ad, "_current_level", 0) >= 0:         # (-1: nobody is taking forward derivatives)
+        _refuse_tangents(q, kv, weights, out, lse)
     index, qs = q.get_device(), q.stride()
     key = (q.shape, qs, q.dtype, index,
            kv.shape, kv.stride(), kv.dtype, kv.get_device(),
