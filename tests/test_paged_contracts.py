@@ -8,6 +8,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 from tests.test_paged_refusals import FAKE, attn_args, attn_metas, geom, meta
 from world_engine_b200 import PagedSlab, _lib, ops
+from world_engine_b200._lib import PagedGeom
 from world_engine_b200.csrc import build as csrc_build
 
 
@@ -65,3 +66,16 @@ def test_ops_refuse_what_has_a_tangent():
                 call()
         with pytest.raises(RuntimeError, match="no CPU path"):
             slab.append(x, x)
+
+
+def test_a_budgeted_slab_costs_what_its_budget_needs(lib):
+    slab = PagedSlab(2, 2, 64, torch.bfloat16, 16, 40, 4096, keep=100, sink=2, recent=8, device="cpu")
+    assert slab.table.shape[1] == slab.max_pages == 7
+    g = PagedGeom(2, 2, 64, 16, 40, slab.max_pages, _lib.BF16, 0, *slab.kv.stride()[:4], slab.table.stride(0))
+    assert lib.we_b200_paged_evict_workspace_bytes(ctypes.byref(g), 1, 100) == 0
+    slab.reserve(0, 4096)                        # as before, but a session under a budget gets no more than that needs
+    assert slab.room(0) == 112 and slab.free_pages == 33
+    slab.reserve(0, 100)
+    assert slab.free_pages == 33
+    with pytest.raises(ValueError, match="at most"):
+        slab.reserve(1, 4097)

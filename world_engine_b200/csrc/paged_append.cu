@@ -690,9 +690,11 @@ static EvictPlan evict_plan(const we_b200_paged_geom& g, int32_t T, int32_t keep
   // 12.9 with 512, 13.6 with 1024, whose scans over the block take longer; 512 heads of 2064: 12.5 us, 16.4 with 512)
   r.threads = units > 2 * sm_count() ? 256 : 512;
   r.cluster = cluster_for(units, usual, kEvictPerCta, sm_count());
-  const int64_t fit = ((usual + r.cluster - 1) / r.cluster + 3) & ~3ll;
-  r.fit = static_cast<int>(fit < kMaxFit ? fit : kMaxFit);
+  // (to the end of the budget's last page: a table that has no more pages needs no lists in the workspace)
   const int64_t most = static_cast<int64_t>(g.max_pages) * g.page + T;
+  const int64_t whole = (static_cast<int64_t>(keep) + g.page - 1) / g.page * g.page + T;
+  const int64_t fit = ((whole + r.cluster - 1) / r.cluster + 3) & ~3ll;
+  r.fit = static_cast<int>(fit < kMaxFit ? fit : kMaxFit);
   const int64_t slice = ((most + r.cluster - 1) / r.cluster + 3) & ~3ll;
   r.list = slice <= r.fit ? 0 : slice;
   r.chunk = 2 * r.list + 2 * ((r.list + 31) >> 5);

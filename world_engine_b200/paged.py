@@ -28,7 +28,10 @@ from . import ops
 
 
 class PagedSlab:
-    """One layer's paged K/V caches of `n_sessions` sessions (state as described in include/we_b200.h)."""
+    """One layer's paged K/V caches of `n_sessions` sessions (state as described in include/we_b200.h).
+
+    A budget (`keep`) also sets the width of the table, and with it the workspaces of a step: it can be lowered later, not
+    raised."""
 
     def __init__(self, n_sessions: int, H: int, Dh: int, dtype: torch.dtype, page: int, n_pages: int,
                  max_tokens: int, keep: Optional[int] = None, sink: int = 0, recent: int = 0, device="cuda"):
@@ -40,7 +43,9 @@ class PagedSlab:
             raise ValueError("a budget needs 0 <= sink + recent <= keep <= max_tokens")
         self.n_sessions, self.page = n_sessions, page
         self.keep, self.sink, self.recent = keep, sink, recent
-        self.max_pages = -(-max_tokens // page)
+        # (what a session can come to hold: workspaces are sized by the width of the table)
+        self.max_tokens = max_tokens
+        self.max_pages = -(-(max_tokens if keep is None else keep) // page)
         self.kv = torch.zeros(2, n_pages, H, page, Dh, dtype=dtype, device=device)
         self.weights = torch.zeros(n_pages, H, page, dtype=torch.float32, device=device)
         self.positions = torch.zeros(n_pages, H, page, dtype=torch.int32, device=device)
@@ -60,10 +65,12 @@ class PagedSlab:
         return len(self._pages[i]) * self.page
 
     def reserve(self, i: int, tokens: int) -> None:
-        """Pages for `tokens` tokens of session i (what it has already counts; none are given back)."""
+        """Pages for `tokens` tokens of session i, under a budget for no more than that (what it has already counts;
+        none are given back)."""
         have, want = self._pages[i], -(-tokens // self.page)
-        if want > self.max_pages:
-            raise ValueError(f"a session holds at most {self.max_pages * self.page} tokens")
+        if want > -(-self.max_tokens // self.page):
+            raise ValueError(f"a session holds at most {-(-self.max_tokens // self.page) * self.page} tokens")
+        want = min(want, self.max_pages)
         if want - len(have) > len(self._free):
             raise RuntimeError(f"the pool has {len(self._free)} free pages, session {i} needs {want - len(have)} more")
         if want <= len(have):
