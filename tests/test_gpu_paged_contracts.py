@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import paged_oracle
-from tests.paged_helpers import Cache, check_attention
+from tests.paged_helpers import Cache, check_attention, half_step
 from world_engine_b200 import PagedSlab, ops
 
 pytestmark = pytest.mark.gpu
@@ -242,3 +242,50 @@ def test_traces_with_permuted_queries():
     assert torch.equal(y, want) and y.stride() == want.stride() and torch.equal(flat, want_flat)
     q = x.transpose(0, 1)
     check_attention(c, q, y)
+
+
+# ------------------------------------------------------------------------------------------------ numbers
+def one_column(c, logits, scale=1.0):
+    """Keys whose only column is the logit (times 1/scale): the logits of q = 1 in that column are exact."""
+    n = len(logits)
+    i = torch.arange(n)
+    pg, row = c.table_h[0, i // c.page].long(), i % c.page
+    k = torch.zeros(n, c.Dh, dtype=c.dtype)
+    k[:, 0] = logits.to(c.dtype)
+    c.kv[0, pg.cuda(), 0, row.cuda()] = k.cuda()
+    c.kv64[0, pg, 0, row] = k.double().numpy()
+    return pg, row, k[:, 0].double()
+
+
+def put_values(c, pg, row, v):
+    c.kv[1, pg.cuda(), 0, row.cuda()] = v.cuda()
+    c.kv64[1, pg, 0, row] = v.double().numpy()
+
+
+def ones_in_column_0(c, G=1, x=1.0):
+    q = torch.zeros(1, G, 1, c.Dh, dtype=c.dtype, device="cuda")
+    q[..., 0] = x
+    return q
+
+
+@pytest.mark.parametrize("G", [1, 3, 16])
+@pytest.mark.parametrize("n,drop", [(100000, 25.6), (100000, 31.0), (2000, 24.3)])
+def test_many_small_weights_count_in_fp16(G, n, drop):
+    """One token takes nearly all of the weight and its value is 0; all others have weights that 16 bits cannot hold on
+    their own, and value 1: the output is what they have in all.  The logits are exact (multiples of 2^-4 below 32); their
+    log2 e multiple is off by 2 * 2^-24 * 45 < 2^-17 (natural: the weights by that), sums as above."""
+    c = Cache(1, 1, 64, 32, -(-n // 32), F16, seed=4, lens=[n])
+    x0 = round(drop * np.log(2) * 16) / 16
+    for first in (0, n - 1, n // 2):
+        logits = torch.full((n,), -x0)
+        logits[first] = 0.0
+        pg, row, x = one_column(c, logits)
+        v = torch.ones(n, 64, dtype=F16)
+        v[first] = 0.0
+        put_values(c, pg, row, v)
+        p = torch.exp(x)
+        p /= p.sum()
+        want = float(p.sum() - p[first])
+        got = ops.paged_attn(ones_in_column_0(c, G), c.kv, c.table, c.lens, scale=1.0).double()
+        tol = want * (half_step(F16) + 2.0 ** -15 + (n / 16 + 64) * 2.0 ** -23) + 2.0 ** -25
+        assert float((got - want).abs().max()) <= tol

@@ -21,7 +21,10 @@
 //              exceeds it by more than 8 (then O is rescaled in tensor memory), so a tile costs one vote among the
 //              128 threads and no reduction.  P goes to shared memory as the sum of two 16-bit numbers in two
 //              columns: the second column costs nothing (N is at least 16) and leaves the weights accurate to 2^-16
-//              instead of 2^-8.  A token's columns lie next to each other (P is an MN-major operand): one or two
+//              instead of 2^-8 (fp16: 2^-22 instead of 2^-11, down to 2^-43 of the largest weight: its exponents end
+//              soon, so the reference lies 7 below the largest logit and the second number is held times 2^12; without
+//              that, tokens of less than 2^-25 of the largest weight counted for nothing, however many they were).
+//              A token's columns lie next to each other (P is an MN-major operand): one or two
 //              16-byte stores per token.
 //   warp 8     walks the run and publishes the segments, one ahead of the one being loaded: what to read, its first
 //              pages, its Q rows; takes further runs
@@ -47,7 +50,13 @@ constexpr uint32_t kTmemColumns = 128;
 constexpr uint32_t kColO = 64;             // + 32 per group
 constexpr float kFloor = -1.0e38f;         // the reference before the first logit
 constexpr int kMaxGroup = 16;              // query heads per unit
-constexpr float kRaise = 8.0f;             // log2 units by which a logit may exceed the reference
+constexpr float kRaise = 8.0f;             // log2 units by which a logit may exceed the largest so far
+// fp16: weights are held times 2^7 (2^15 at most, after a rise that is not followed), what is left of them by the first
+// rounding (8 at most) times 2^12 (2^15 at most)
+template <bool BF16>
+constexpr float kAbove = BF16 ? 0.f : 7.f;
+template <bool BF16>
+constexpr float kLowScale = BF16 ? 1.f : 4096.f;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinTokens = 4 * kJoinThreads;
 constexpr int kWholeUnitTokens = 128;      // sessions this short are never split
@@ -681,7 +690,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
           e[g] = x[g] - m[g];
           over = fmaxf(over, e[g]);
         }
-        if (bar_any(2 + grp, 128, over > kRaise)) {
+        if (bar_any(2 + grp, 128, over > kRaise + kAbove<BF16>)) {
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
             const float t = warp_max(x[g]);
@@ -691,7 +700,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
           float f[GP];
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
-            const float t = fmaxf(fmaxf(fmaxf(my_max[g], my_max[16 + g]), fmaxf(my_max[32 + g], my_max[48 + g])), m[g]);
+            const float top = fmaxf(fmaxf(my_max[g], my_max[16 + g]), fmaxf(my_max[32 + g], my_max[48 + g]));
+            const float t = fmaxf(top - kAbove<BF16>, m[g]);
             f[g] = t == m[g] ? 1.f : exp2_fast(m[g] - t);
             m[g] = t;
             l[g] *= f[g];
@@ -721,14 +731,14 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
         }
         if constexpr (GP == 1) {
           const uint16_t hi = narrow<BF16>(e[0]);
-          words[0] = hi | (static_cast<uint32_t>(narrow<BF16>(e[0] - widen<BF16>(hi))) << 16);
+          words[0] = hi | (static_cast<uint32_t>(narrow<BF16>((e[0] - widen<BF16>(hi)) * kLowScale<BF16>)) << 16);
         } else {
 #pragma unroll
           for (int g = 0; g < GP; g += 2) {
             const uint32_t hi = narrow2<BF16>(e[g], e[g + 1]);
             words[g / 2] = hi;
-            words[(GP + g) / 2] = narrow2<BF16>(e[g] - widen<BF16>(static_cast<uint16_t>(hi)),
-                                                e[g + 1] - widen<BF16>(static_cast<uint16_t>(hi >> 16)));
+            words[(GP + g) / 2] = narrow2<BF16>((e[g] - widen<BF16>(static_cast<uint16_t>(hi))) * kLowScale<BF16>,
+                                                (e[g + 1] - widen<BF16>(static_cast<uint16_t>(hi >> 16))) * kLowScale<BF16>);
           }
         }
         if (it >= 2) mbar_wait(&pv_done[grp], ((it - 2) >> 1) & 1, s_abort);      // the P before was read
@@ -783,7 +793,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm, const PagedAttnParams 
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
         // (an infinite value times a low part, which may be 0 or negative, is none of the formula's terms)
-        const float y = __uint_as_float(lo[g]);
+        const float y = __uint_as_float(lo[g]) * (1.f / kLowScale<BF16>);
         o[g] = __uint_as_float(hi[g]) + (fabsf(y) < INFINITY ? y : 0.f);
       }
       __syncwarp();
