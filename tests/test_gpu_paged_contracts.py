@@ -268,6 +268,38 @@ def ones_in_column_0(c, G=1, x=1.0):
     return q
 
 
+def narrowed(x, dtype):
+    return x.to(dtype).double()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n", [300, 1500])
+def test_weights_are_held_in_more_than_16_bits(dtype, n):
+    """Values chosen against the rounding of the weights: each has the sign of what rounding its weight to 16 bits would
+    lose, and half of them cancel the other half.  Logits lie in one column, so they are exact but for the scaling: with
+    |x| <= 6, x log2 e is off by 6 * 1.5 * 2^-23 < 2^-19 and e^x by 2^-19 of itself, 2^x of the GPU by 2^-21, twice for
+    the normalisation (2^-17 in all).  A weight as the sum of two 16-bit numbers is off by half a step of half a step.
+    Sums are held in fp32, 16 products to an addition that may truncate, in runs joined in fp32: at most n / 16 + 64
+    steps of 2^-23."""
+    c = Cache(1, 1, 64, 16, -(-n // 16), dtype, seed=3, lens=[n])
+    g = torch.Generator().manual_seed(n)
+    logits = -6 * torch.rand(n, generator=g)
+    logits[::64] = 0.0                                   # the reference of every tile
+    pg, row, x = one_column(c, logits)
+    e = torch.exp(x)
+    lost = e - narrowed(e, dtype)
+    v = torch.where(lost >= 0, 1.0, -1.0)[:, None].expand(n, 64).to(dtype).contiguous()
+    put_values(c, pg, row, v)
+    p = e / e.sum()
+    want, spread = float((p * v[:, 0].double()).sum()), 1.0
+    u = half_step(dtype)
+    tol = (2.0 ** -17 + u * u + (n / 16 + 64) * 2.0 ** -23) * spread + u * abs(want)
+    single = float((narrowed(e, dtype) * v[:, 0].double()).sum() / e.sum())
+    assert abs(single - want) > 1.5 * tol                # what the tolerance is there to see
+    got = ops.paged_attn(ones_in_column_0(c), c.kv, c.table, c.lens, scale=1.0).double()
+    assert float((got - want).abs().max()) <= tol
+
+
 @pytest.mark.parametrize("G", [1, 3, 16])
 @pytest.mark.parametrize("n,drop", [(100000, 25.6), (100000, 31.0), (2000, 24.3)])
 def test_many_small_weights_count_in_fp16(G, n, drop):
