@@ -321,3 +321,16 @@ def test_many_small_weights_count_in_fp16(G, n, drop):
         got = ops.paged_attn(ones_in_column_0(c, G), c.kv, c.table, c.lens, scale=1.0).double()
         tol = want * (half_step(F16) + 2.0 ** -15 + (n / 16 + 64) * 2.0 ** -23) + 2.0 ** -25
         assert float((got - want).abs().max()) <= tol
+
+def test_logits_at_the_far_end_of_the_range():
+    # logits of -1.5e38 to -2e38: the softmax goes by their differences all the same
+    n = 300
+    c = Cache(1, 1, 64, 16, 20, BF16, seed=5, lens=[n])
+    logits = -torch.linspace(1.5e19, 2e19, n)
+    pg, row, _ = one_column(c, logits)
+    out = ops.paged_attn(ones_in_column_0(c, 1, 1e19), c.kv, c.table, c.lens, scale=1.0)
+    top = (c.kv64[0, pg, 0, row][:, 0] == c.kv64[0, pg, 0, row][:, 0].max())
+    want = c.kv64[1, pg, 0, row][top].mean(axis=0)       # of equal ones the mean
+    spread = np.abs(c.kv64[1, pg, 0, row][top]).mean(axis=0)
+    got = out[0, 0, 0].double().cpu().numpy()
+    assert np.all(np.abs(got - want) <= half_step(BF16) * np.abs(want) + 2.0 ** -15 * spread)

@@ -48,7 +48,7 @@ constexpr int kSegs = 3;                   // segments in flight
 constexpr int kBufs = 4;                   // S buffers
 constexpr uint32_t kTmemColumns = 128;
 constexpr uint32_t kColO = 64;             // + 32 per group
-constexpr float kFloor = -1.0e38f;         // the reference before the first logit
+constexpr float kFloor = -3.4028234e38f;   // the reference before the first logit: no finite one lies below
 constexpr int kMaxGroup = 16;              // query heads per unit
 constexpr float kRaise = 8.0f;             // log2 units by which a logit may exceed the largest so far
 // fp16: weights are held times 2^7 (2^15 at most, after a rise that is not followed), what is left of them by the first
