@@ -1,5 +1,9 @@
 """What the paged cache promises about calls that go wrong or sit out: tokens without a page, sessions without a new token,
 the ends of the number range, reports across graph replays."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -11,6 +15,7 @@ from world_engine_b200 import PagedSlab, ops
 pytestmark = pytest.mark.gpu
 
 BF16, F16 = torch.bfloat16, torch.float16
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(autouse=True)
@@ -334,3 +339,33 @@ def test_logits_at_the_far_end_of_the_range():
     spread = np.abs(c.kv64[1, pg, 0, row][top]).mean(axis=0)
     got = out[0, 0, 0].double().cpu().numpy()
     assert np.all(np.abs(got - want) <= half_step(BF16) * np.abs(want) + 2.0 ** -15 * spread)
+
+# ------------------------------------------------------------------------------------------------ reports
+CHILD = """
+import torch
+from world_engine_b200 import PagedSlab, ops
+slab = PagedSlab(1, 2, 64, torch.bfloat16, 16, 4, 32)
+slab.reserve(0, 32)
+x = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):                 # the first calls of the process
+    slab.append_and_attend(x, x, x)
+dev = torch.device("cuda")
+ops.check_status(dev)
+page = int(slab.table[0, 0])
+slab.table[0, 0] = -1
+graph.replay()
+slab.table[0, 0] = page
+graph.replay()
+try:
+    ops.check_status(dev)
+except RuntimeError as e:
+    print("reported", e)
+ops.check_status(dev)
+"""
+
+
+def test_a_report_outlives_the_next_replay():
+    r = subprocess.run([sys.executable, "-c", CHILD], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    assert "reported" in r.stdout and "page" in r.stdout

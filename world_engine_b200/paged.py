@@ -52,6 +52,9 @@ class PagedSlab:
         self.table = torch.full((n_sessions, self.max_pages), -1, dtype=torch.int32, device=device)  # -1: no page
         self.lens = torch.zeros(n_sessions, H, dtype=torch.int32, device=device)
         self.next_pos = torch.zeros(n_sessions, H, dtype=torch.int32, device=device)
+        if self.kv.is_cuda:
+            # made here, not within the first captured step: a graph that holds its making clears it at every replay
+            ops.status_word(self.kv.device)
         self._free: List[int] = list(range(n_pages - 1, -1, -1))
         self._pages: List[List[int]] = [[] for _ in range(n_sessions)]
 
