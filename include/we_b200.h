@@ -384,7 +384,7 @@ WE_B200_API int we_b200_paged_attn(const we_b200_paged_attn_args* args_host, int
 WE_B200_API size_t we_b200_paged_attn_workspace_bytes(const we_b200_paged_geom* geom_host, int32_t Hq,
                                                       int uses);
 
-/* Number of kernels the previous three entry points have launched in this
+/* Number of kernels the entry points above have launched in this
  * process (diagnostic counter for benchmarks; relaxed atomics). */
 WE_B200_API uint64_t we_b200_launch_count(void);
 

@@ -369,3 +369,36 @@ def test_a_report_outlives_the_next_replay():
     r = subprocess.run([sys.executable, "-c", CHILD], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr
     assert "reported" in r.stdout and "page" in r.stdout
+
+
+# ------------------------------------------------------------------------------------------------ arguments that steps rarely give
+@pytest.mark.parametrize("lens,T", [([40, 50], 6), ([10, 0], 6), ([50, 50], 0)])
+def test_eviction_into_other_counts(lens, T):
+    c = Cache(2, 3, 64, 16, 4, BF16, seed=T, lens=lens)
+    (k, v, w), (k64, v64, w64) = c.new(T, seed=3, with_weights=True)
+    held, given = c.lens.clone(), c.next_pos.clone()
+    lens_out, next_pos_out = torch.full_like(held, -7), torch.full_like(held, -7)
+    ops.paged_append_evict_(c.kv, c.table, c.lens, c.next_pos, k, v, c.weights, c.positions, 44, 2, 9, w_new=w, lens_out=lens_out,
+                            next_pos_out=next_pos_out)
+    assert torch.equal(c.lens, held) and torch.equal(c.next_pos, given)
+    paged_oracle.append_evict(c.kv64, c.table64, c.lens64, c.next64, k64, v64, None, c.w64, c.pos64, 44, 2, 9, w64)
+    c.lens, c.next_pos = lens_out, next_pos_out
+    c.assert_same_state()
+
+
+def test_a_prompt_with_weights_into_a_budgeted_slab():
+    # w_new as a view with strides of its own, a padded batch
+    S, H, Dh, page, keep, T = 3, 2, 128, 16, 30, 100
+    slab = PagedSlab(S, H, Dh, F16, page, 8, 4096, keep=keep, sink=2, recent=6)
+    for s in range(S):
+        slab.reserve(s, 4096)
+    c = Cache(S, H, Dh, page, 2, F16, lens=[0] * S)
+    (k, v, w), (k64, v64, w64) = c.new(T, seed=4, with_weights=True)
+    n_new = torch.tensor([100, 17, 31], dtype=torch.int32)
+    kv64, w_64, pos64 = (x.cpu().numpy().copy() for x in (slab.kv.double(), slab.weights.double(), slab.positions))
+    lens64, next64 = np.zeros((S, H), np.int32), np.zeros((S, H), np.int32)
+    slab.append(k, v, n_new.cuda(), w.transpose(0, 2).contiguous().transpose(0, 2))
+    paged_oracle.append_evict(kv64, slab.table.cpu().numpy(), lens64, next64, k64, v64, n_new, w_64, pos64, keep, 2, 6, w64)
+    assert np.array_equal(slab.kv.double().cpu().numpy(), kv64) and np.array_equal(slab.weights.double().cpu().numpy(), w_64)
+    assert np.array_equal(slab.positions.cpu().numpy(), pos64) and np.array_equal(slab.lens.cpu().numpy(), lens64)
+    assert lens64.tolist() == [[30, 30], [17, 17], [30, 30]]
