@@ -165,14 +165,15 @@ __device__ __forceinline__ void move_tokens(const PagedAppendParams& p, int s, i
 }
 
 // 16-byte vectors of K and of V that a thread has under way (and the pages of its next ones).  Prompts of 142000 tokens
-// (146 MB read and written): 28.1 us with two and six CTAs on an SM, 5.2 TB/s or 0.79 of the measured copy; 30.3 with
-// five, 34.8 with one vector and eight CTAs, 30.9 with four and four.  Bound by the latency of the rows' loads.
+// (146 MB read and written), without the look at the pages: 28.1 us with two and six CTAs on an SM, 30.3 with five, 34.8 with one
+// vector and eight CTAs, 30.9 with four and four.  With it 29.2 us, 5.0 TB/s or 0.76 of the measured copy.  Bound by the
+// latency of the table's and the rows' loads.
 constexpr int kRows = 2;
 
 //
 // kStep: one token per session (64 threads).  Its page is looked up once, while its row is on its way, and thread 0 of the
 // unit, which copies a part of it, knows whether it had one: 64 sessions x 16 heads take 2.3 us, 2.75 with the general look.
-// The general kernel looks at the pages of all its tokens first (1.1 us of the prompts' 29.5): what lies behind the first
+// The general kernel looks at the pages of all its tokens first (1 us of the prompts' 29.2): what lies behind the first
 // missing page is not to be written, however many pages follow it.
 template <bool kStep>
 __global__ void __launch_bounds__(kStep ? 64 : kAppendThreads, kStep ? 16 : 6) paged_append_kernel(const PagedAppendParams p) {
