@@ -226,8 +226,9 @@ def test_a_step_that_some_sessions_sit_out(budget, compiled):
                 assert torch.all(y[s] == 0)
             else:
                 z = alone[s].append_and_attend(q[s:s + 1], k[s:s + 1], v[s:s + 1]).float()
-                # (cut into other runs: the sums are added up in another order)
-                assert torch.allclose(y[s].float(), z[0], rtol=2 ** -6, atol=2 ** -10)
+                # (cut into other runs, so sums are added up in another order: two roundings to bf16 and 2^-13 of the
+                # largest values in between, where weights are held to 2^-16)
+                assert torch.allclose(y[s].float(), z[0], rtol=2 ** -7, atol=2 ** -11)
     for s in range(3):
         assert torch.equal(every.lens[s], alone[s].lens[0]) and torch.equal(every.next_pos[s], alone[s].next_pos[0])
         assert torch.isfinite(every.weights).all()
@@ -247,6 +248,33 @@ def test_traces_with_permuted_queries():
     assert torch.equal(y, want) and y.stride() == want.stride() and torch.equal(flat, want_flat)
     q = x.transpose(0, 1)
     check_attention(c, q, y)
+
+
+def test_a_captured_step_whose_sessions_come_and_go():
+    def slab():
+        x = PagedSlab(4, 2, 128, BF16, 16, 16, 64, keep=40, sink=1, recent=4)
+        for s in range(4):
+            x.reserve(s, 40)
+        return x
+    eager, graphed = slab(), slab()
+    g = torch.Generator().manual_seed(8)
+    steps = [[torch.randn(4, n, 1, 128, generator=g).to(BF16).cuda() for n in (4, 2, 2)] +
+             [torch.randint(0, 2, (4,), generator=g, dtype=torch.int32).cuda()] for _ in range(60)]
+    held = [x.clone() for x in steps[0]]
+    held[3].zero_()
+    graphed.append_and_attend(*held)                     # (everybody sits out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = graphed.append_and_attend(*held)
+    for i, step in enumerate(steps):
+        want = eager.append_and_attend(*step)
+        for a, b in zip(held, step):
+            a.copy_(b)
+        graph.replay()
+        assert torch.equal(y, want), i
+        assert torch.all(y[step[3] == 0] == 0)
+    for name in ("kv", "weights", "positions", "lens", "next_pos"):
+        assert torch.equal(getattr(eager, name), getattr(graphed, name)), name
 
 
 # ------------------------------------------------------------------------------------------------ numbers

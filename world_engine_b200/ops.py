@@ -463,7 +463,8 @@ def paged_attn(q: torch.Tensor, kv: torch.Tensor, table: torch.Tensor, lens: tor
     (summed over the query heads of its kv head) is added to it in place; `lse` (float32 `[S, Hq]`, contiguous)
     receives the logarithm of the softmax sum.  A kv head that holds nothing gives 0 and -inf.  So does a
     session that sits out (`n_new[s] < 1`, int32 `[S]`, as in a padded append): its weights stay as they are, and
-    neither its cache nor its row of `q` is read.  `out` must not overlap `q`.  Results repeat bit for bit (but for the weights of pages that several sessions share)."""
+    neither its cache nor its row of `q` is read.  `out` must not overlap `q`.  Results repeat bit for bit (but for the
+    weights of pages that several sessions share)."""
     if torch.is_grad_enabled():
         _refuse_grad(q, kv, weights, out, lse)
     if getattr(_forward_ad, "_current_level", 0) >= 0:         # (-1: nobody is taking forward derivatives)
