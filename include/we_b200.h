@@ -343,7 +343,8 @@ WE_B200_API int we_b200_paged_append(const we_b200_paged_append_args* args_host,
  * the table names no page for them, those below the budget stay held, with
  * nothing moved there (as many fewer tokens find room), the others are given up.
  * The positions of a kv head's tokens are distinct, as appends make them, so at
- * most `keep` are shielded (of more, the lowest indexes would stay).
+ * most sink + recent are shielded and all of these stay.  Where there is less
+ * room (slots without a page) or there are more, the lowest indexes of them do.
  * The workspace (we_b200_paged_evict_workspace_bytes) needs no initialisation.
  * max_pages * page + T < 2^21.
  */

@@ -100,7 +100,9 @@ def append_evict(kv, table, lens, next_pos, k_new, v_new, n_new, weights, positi
                 if i < held and rows[i] is None:   # a slot without a page: it can neither move nor be filled
                     return (-1 if i < keep else 2, False, 0.0, i)
                 w, pos = rows[i][2], rows[i][3]
-                return (not (pos < sink or pos >= end - recent), not np.isnan(w), 0.0 if np.isnan(w) else -w, i)
+                if pos < sink or pos >= end - recent:
+                    return (0, False, 0.0, i)
+                return (1, not np.isnan(w), 0.0 if np.isnan(w) else -w, i)
             kept = sorted(range(len(rows)), key=order)[:keep]
             stay = set(kept)
             holes = [i for i in range(min(keep, len(rows))) if i not in stay]

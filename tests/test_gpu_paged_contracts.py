@@ -128,6 +128,7 @@ def test_a_long_append_stops_where_its_pages_do():
     ([90, 70], 3, 50, 1, 30, [(0, 1), (0, 4), (1, 3)]),  # the budget was lowered: slots of either side
     ([90, 70], 0, 20, 0, 0, [(0, 2), (0, 3), (0, 4), (0, 5), (1, 0)]),
     ([48, 64], 200, 64, 4, 16, [(0, 0), (1, 3)]),        # a prompt
+    ([64, 48], 79, 64, 4, 30, [(0, 0), (0, 2), (0, 3), (1, 0), (1, 1)]),   # ... fewer slots than shielded tokens
     ([64, 64], 5, 64, 0, 0, [(0, 0), (0, 1), (0, 2), (0, 3)])])   # no page at all
 @pytest.mark.parametrize("with_weights", [False, True])
 def test_eviction_neither_keeps_nor_fills_a_slot_without_a_page(lens, T, keep, sink, recent, blocks, with_weights):
